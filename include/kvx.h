@@ -35,13 +35,15 @@ extern "C" {
 #endif
 
 /*
+ * Version 3: the operators around an e4m3 KV cache (rotary positions, cache
+ * write, attention, the weights of cached tokens, their choice and compaction).
  * Version 2: kvx_upload and kvx_cache_dma_counters; allocation-free saves of
  * different caches on one device ordered by a per-device event; staging areas
  * replaced on a split-stream cache order both copy streams; waited one- and
  * two-block restores may run on the caller's stream; synchronize/destroy wait
  * for those; set_staging rejects overlapping split areas; KVX_DEBUG_* flags.
  */
-#define KVX_ABI_VERSION 2
+#define KVX_ABI_VERSION 3
 
 /* Error codes (negative); positive values are hipError_t. */
 #define KVX_OK 0
@@ -170,6 +172,132 @@ int kvx_gather_tokens_fp8(const void* pool, const kvx_block_layout* layout, cons
 int kvx_scatter_tokens_fp8(void* pool, const kvx_block_layout* layout, const int32_t* block_table_host,
                            int32_t table_len, int64_t num_rows, const void* payload, const void* scales,
                            void* stream);
+
+/*
+ * Operators around an e4m3 KV cache: a layer's keys and values held as e4m3fn
+ * codes in a paged pool [NB, BS, H, hd] with one fp32 scale for each group of
+ * G tokens of a block and KV head, [NB, BS / G, H]. The reference keeps its
+ * pool in the model's type; these have no counterpart there beyond the calls
+ * that nanovllm/layers/attention.py:59-74 makes around its pool.
+ *
+ * Limits (KVX_E_UNSUPPORTED): G a multiple of 16, at most 1024; hd a multiple
+ * of 16, at most 256. Codes and the rows of queries, keys and values start on
+ * 16 bytes. Block ids outside [0, NB) are read as blocks that hold nothing and
+ * are never written. All calls only queue kernels and can be captured.
+ */
+#define KVX_DTYPE_BF16 0
+#define KVX_DTYPE_FP16 1
+#define KVX_DTYPE_FP32 2
+
+typedef struct kvx_fp8_cache {
+  void* k_codes;   /* e4m3fn [NB, BS, H, hd], contiguous */
+  void* v_codes;   /* may be NULL where only keys are read */
+  float* k_scales; /* [NB, BS / G, H], contiguous */
+  float* v_scales;
+  int32_t num_blocks; /* NB */
+  int32_t block_size; /* BS */
+  int32_t group_size; /* G, divides BS */
+  int32_t num_heads;  /* H */
+  int32_t head_dim;   /* hd */
+} kvx_fp8_cache;
+
+/*
+ * The sequences of a call (device arrays). Sequence b's cached token t is in
+ * block block_tables[b * table_stride + t / BS]; context_lens[b] of them are
+ * cached, this call's own among them (lengths beyond the table's count as what
+ * it holds). Its queries are the rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
+ * the call, or row b where cu_seqlens is NULL, and are its last tokens: row i of
+ * n sees the cached tokens 0 .. context - n + i.
+ */
+typedef struct kvx_paged_batch {
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  const int32_t* cu_seqlens; /* NULL: one row a sequence */
+  int64_t table_stride;      /* elements */
+  int32_t table_width;       /* blocks of a table */
+  int32_t num_seqs;
+  int32_t max_seqlen; /* the most rows of a sequence; a launch is sized by it, and longer ones are computed too */
+  int32_t num_tokens; /* rows of the call; those of no sequence are not written */
+} kvx_paged_batch;
+
+/*
+ * Rotary positions: the first rotary_dim elements of each head of query and
+ * key rotated, in pairs (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1),
+ * by positions[token] * frequencies[i] and multiplied by `magnitude`; the rest
+ * copied. An output may be its input; other overlaps are not allowed. Strides
+ * are between tokens, in elements; a token's heads are packed. positions:
+ * int32 or int64 (position_bytes 4 or 8); frequencies: rotary_dim / 2 doubles,
+ * radians a position. Either tensor may have no heads.
+ */
+int kvx_rotary_embed(const void* query, int64_t query_stride, const void* key, int64_t key_stride, void* query_out,
+                     int64_t query_out_stride, void* key_out, int64_t key_out_stride, const void* positions,
+                     int32_t position_bytes, const double* frequencies, int64_t num_tokens, int32_t query_heads,
+                     int32_t key_heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float magnitude,
+                     int32_t dtype, void* stream);
+
+/*
+ * Slot-mapped write into an e4m3 cache; slots as kvx_store_kvcache's. A
+ * group's scale becomes the least power of two s >= 2^-100 with |x| / s <= 448
+ * for all finite x that the call writes into it, and codes are x / s to the
+ * nearest (infinities +-448, NaN as NaN). Where the call does not write the
+ * group's first slot, the group goes on: its scale is the larger of that and
+ * the one it had, and if that grew, its other rows are encoded anew. Where it
+ * does, the group starts over, and rows that the call does not write hold
+ * nothing. The tokens of one group stand together in the call; of two with one
+ * slot the later one is stored.
+ */
+int kvx_store_kvcache_fp8(const kvx_fp8_cache* cache, const void* key, int64_t key_stride, const void* value,
+                          int64_t value_stride, int32_t dtype, const int32_t* slot_mapping, int64_t num_tokens,
+                          void* stream);
+
+/*
+ * Causal attention over an e4m3 cache: out[row, head] = softmax(softmax_scale *
+ * q . K) V over the tokens that the row sees, lse the logarithm of the sum of
+ * exp(scores) (NULL: not written); 0 and -infinity for a row that sees none.
+ * query_heads is a multiple of H; head h reads KV head h / (query_heads / H).
+ * out: [num_tokens, query_heads, hd] of the query's type, lse: [num_tokens,
+ * query_heads]. `workspace`: as many bytes as kvx_attention_fp8_workspace
+ * gives, used until the queued work is done.
+ */
+int kvx_attention_fp8_workspace(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, int32_t query_heads,
+                                int64_t* bytes);
+int kvx_attention_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, const void* query,
+                      int64_t query_stride, int32_t query_heads, int32_t dtype, float softmax_scale, void* out,
+                      float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The weight that each cached token received: out[b, h, t] = weights[b, h, t]
+ * (0 where NULL) + the sum of exp(softmax_scale * q . K_t - lse) over the rows
+ * of sequence b that see t and the query heads of KV head h. weights and out:
+ * [num_seqs, H, width], out may be weights; tokens at or past `width` are
+ * dropped. lse as kvx_attention_fp8 gives it. The sums have a fixed order.
+ */
+int kvx_attention_weights_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, const void* query,
+                              int64_t query_stride, int32_t query_heads, int32_t dtype, float softmax_scale,
+                              const float* lse, const float* weights, float* out, int64_t width, void* stream);
+
+/*
+ * The tokens of each (sequence, KV head) to keep: of n = min(context, width)
+ * all, where n <= keep; else the last `recent` (at most keep) and the keep -
+ * recent of the others with the largest weights, of equal ones the earliest
+ * (NaN below all). indices: [num_seqs, num_heads, keep] ascending, then -1;
+ * kept: their weights, then 0; counts: [num_seqs], min(n, keep).
+ */
+int kvx_select_tokens(const float* weights, const int32_t* context_lens, int32_t num_seqs, int32_t num_heads,
+                      int64_t width, int32_t keep, int32_t recent, int32_t* indices, int32_t* counts, float* kept,
+                      void* stream);
+
+/*
+ * Moves the tokens indices[b, h, 0 .. counts[b]) of each KV head, in that
+ * order, to positions 0, 1, ... of the blocks to_tables[b * to_stride ..], which
+ * may be no block that `from` reads or that to_tables names twice. Each group
+ * written gets the scale that kvx_store_kvcache_fp8 would give its values; an
+ * index that is no cached token gives zeros. Of `from`, the query rows are not
+ * used, and context_lens may be NULL (all that its tables hold).
+ */
+int kvx_compact_kvcache_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* from, const int32_t* indices,
+                            const int32_t* counts, int32_t keep, const int32_t* to_tables, int64_t to_stride,
+                            int32_t to_width, void* stream);
 
 /*
  * Copy engine: the stream/event half of CPUBlockCache

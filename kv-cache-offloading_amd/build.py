@@ -12,7 +12,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = [HERE / "csrc" / "kvx_kernels.hip", HERE / "csrc" / "kvx_capi.hip"]
+SOURCES = [HERE / "csrc" / name for name in ("kvx_kernels.hip", "kvx_capi.hip", "kvx_step_kernels.hip",
+                                             "kvx_attention.hip", "kvx_step_capi.hip")]
 OUTPUT = HERE / "kvx" / "libkvx.so"
 BIND_SOURCE = HERE / "csrc" / "kvx_bind.cpp"
 BIND_OUTPUT = HERE / "kvx" / "_bind.so"

@@ -1,0 +1,625 @@
+// Attention over a paged e4m3 KV cache, and the weight that each cached token
+// received, on CDNA4's matrix cores.
+//
+// Layout of a wave's work: 32 keys a step against 16 * kTiles query rows (a
+// row is a query token and one of the query heads that share the KV head).
+// Both products keep the query rows in the lanes:
+//   S^T = K Q^T   mfma 16x16x32: A = 16 keys, B = 16 query rows; lane (c, g),
+//                 c = lane % 16, g = lane / 16, gets row c's scores of keys 4 g + i
+//   O^T = V^T P^T mfma 16x16x32 over the step's 32 keys: lane (c, g)'s P values
+//                 are, without a move, the B operand, if the contraction takes
+//                 the keys in the order 4 g + i of the first 16, then of the
+//                 second. V^T's operand then needs, for one column of the
+//                 head, the codes of those 8 keys: each lane loads them for
+//                 head_dim / 16 adjacent columns and transposes bytes in registers.
+// So neither K, V, S nor P passes through LDS. The codes become bf16 (or fp16)
+// values in registers, which hold every e4m3 value exactly; K's scale is
+// applied to the scores and V's to P, in fp32.
+//
+// Softmax statistics, sums and outputs are fp32 until the last rounding. P is
+// rounded to bf16 for the second product. Where that product is not what bounds
+// the kernel (few query rows) or the query is fp16, the rounding's remainder is
+// added as a second bf16 operand, which leaves P with 16 bits.
+#include "kvx_step.h"
+
+namespace kvx {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kStep = 32;  // keys
+
+template <int kType>
+struct Query;
+template <>
+struct Query<KVX_DTYPE_BF16> {
+  using T = __bf16;
+  using Vec = bf16x8;
+  static __device__ __forceinline__ f32x4 mfma(Vec a, Vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pair(uint32_t codes, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));
+  }
+};
+template <>
+struct Query<KVX_DTYPE_FP16> {
+  using T = _Float16;
+  using Vec = f16x8;
+  static __device__ __forceinline__ f32x4 mfma(Vec a, Vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pair(uint32_t codes, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false));
+  }
+};
+
+// Eight codes (two words) as an operand of the query's type.
+template <typename Q>
+__device__ __forceinline__ typename Q::Vec decode8(uint32_t lo, uint32_t hi) {
+  const u32x4 w = {Q::pair(lo, false), Q::pair(lo, true), Q::pair(hi, false), Q::pair(hi, true)};
+  return __builtin_bit_cast(typename Q::Vec, w);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const f32x2 v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
+// The largest (sum) of the values of the four lanes that hold one query row.
+__device__ __forceinline__ float rows_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Rows x[0..3] of four bytes each -> their columns.
+__device__ __forceinline__ void transpose4(const uint32_t* x, uint32_t* out) {
+  const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);  // bytes 0, 0', 1, 1'
+  const uint32_t b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);  // bytes 2, 2', 3, 3'
+  const uint32_t c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+  const uint32_t d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// 16 keys that lie in one block and under one scale: where their rows begin,
+// or nothing where the keys are past the context or their block is no block.
+struct Tile {
+  int64_t row;   // slot * heads + head of the first key
+  int64_t scale; // element of the scales
+  bool there;
+};
+__device__ __forceinline__ Tile tile_at(const Fp8Cache& c, const int32_t* table, int key, int context, int head) {
+  Tile t = {0, 0, false};
+  if (key >= context) return t;
+  const int nth = c.block_of(key), in = key - nth * c.block_size;
+  const int id = __builtin_amdgcn_readfirstlane(table[nth]);
+  if (id < 0 || id >= c.num_blocks) return t;
+  t.row = ((int64_t)id * c.block_size + in) * c.heads + head;
+  t.scale = ((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head;
+  t.there = true;
+  return t;
+}
+
+// kHd: head_dim rounded up to 64, 128 or 256; the columns past head_dim are
+// zeros. kTiles query tiles of 16 rows a wave; kRowWaves of the workgroup's waves
+// take rows of their own, and the others share those and split the keys.
+template <int kType, int kHd, int kTiles, int kRowWaves, int kParts>
+__global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
+  using Q = Query<kType>;
+  using T = typename Q::T;
+  using Vec = typename Q::Vec;
+  constexpr int kKeyWaves = kWaves / kRowWaves;
+  constexpr int kChunks = kHd / 64;    // 64 columns of K: one 16-byte load a lane
+  constexpr int kCols = kHd / 16;      // columns of V a lane loads, transposes and accumulates
+  constexpr int kRows = 16 * kTiles;
+  const Fp8Cache& cache = a.cache;
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row_wave = wave % kRowWaves, key_wave = wave / kRowWaves;
+
+  // Workgroup -> (sequence, KV head), query tile, split. Neighbouring
+  // workgroups take different heads, so that an XCD keeps to few of them.
+  const int pairs = a.batch.num_seqs * cache.heads;
+  const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+  const int split = rest % a.splits;
+  const int tile = a.row_tiles - 1 - rest / a.splits;  // the longest first
+  const int seq = pair / cache.heads, head = pair % cache.heads;
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int context = context_of(a.batch, seq, cache.block_size);
+  const int num_rows = rows.count * a.per_kv;
+  const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
+
+  // A launch covers max_seqlen queries a sequence; longer ones wrap around.
+  for (int tile_row = (tile * kRowWaves + row_wave) * kRows; ; tile_row += a.row_tiles * kRowWaves * kRows) {
+    // With several row waves there is no barrier below; with one, tile_row is the workgroup's.
+    if (tile_row >= num_rows) break;
+    // Query rows and the last key each may see.
+    Vec q[kTiles][2 * kChunks];
+    int last[kTiles], out_row[kTiles];
+    int most = -1;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const int r = tile_row + n * 16 + c;
+      const bool real = r < num_rows;
+      const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
+      last[n] = real ? context - rows.count + nth : -1;
+      out_row[n] = real ? (rows.first + nth) * a.q_heads + head * a.per_kv + sub : -1;
+      most = last[n] > most ? last[n] : most;
+      const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride +
+                     (int64_t)(head * a.per_kv + sub) * cache.head_dim;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int at = k * 64 + g * 16;
+        u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        if (real && at < cache.head_dim) {
+          lo = *reinterpret_cast<const u32x4*>(src + at);
+          hi = *reinterpret_cast<const u32x4*>(src + at + 8);
+        }
+        q[n][2 * k] = __builtin_bit_cast(Vec, lo);
+        q[n][2 * k + 1] = __builtin_bit_cast(Vec, hi);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor(most, d));
+    most = __builtin_amdgcn_readfirstlane(most);
+    // Every key up to here is seen by all of the wave's rows.
+    const int least = context - rows.count + (int)a.per_kv_of(tile_row);
+
+    f32x4 o[kTiles][kCols];
+    float top[kTiles], sum[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      top[n] = -INFINITY;
+      sum[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) o[n][d] = f32x4{0, 0, 0, 0};
+    }
+
+    const int steps = (context + kStep - 1) / kStep;
+    const int per_split = (steps + a.splits - 1) / a.splits;
+    const int first_step = split * per_split;
+    int end_step = min(first_step + per_split, steps);
+    end_step = min(end_step, most / kStep + 1);
+    if (most < 0) end_step = first_step;
+    for (int step = first_step + key_wave; step < end_step; step += kKeyWaves) {
+      const int key0 = step * kStep;
+      const Tile t0 = tile_at(cache, table, key0, context, head);
+      const Tile t1 = tile_at(cache, table, key0 + 16, context, head);
+      const Tile tiles[2] = {t0, t1};
+      // K: lane (c, g) takes columns 16 g .. 16 g + 15 of each 64 of key c's row.
+      f32x4 s[kTiles][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) s[n][t] = f32x4{0, 0, 0, 0};
+        const uint8_t* p = cache.k + (tiles[t].row + (int64_t)c * cache.heads) * cache.head_dim;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          const int at = k * 64 + g * 16;
+          u32x4 w = {0, 0, 0, 0};
+          if (tiles[t].there && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(p + at);
+          const Vec lo = decode8<Q>(w.x, w.y), hi = decode8<Q>(w.z, w.w);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            s[n][t] = Q::mfma(lo, q[n][2 * k], s[n][t]);
+            s[n][t] = Q::mfma(hi, q[n][2 * k + 1], s[n][t]);
+          }
+        }
+      }
+      // V: lane (c, g) takes columns kCols c .. of keys 4 g + i of both tiles.
+      uint32_t v[8][kCols / 4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const Tile& t = tiles[j / 4];
+        const uint8_t* p = cache.v + (t.row + (int64_t)(4 * g + j % 4) * cache.heads) * cache.head_dim + c * kCols;
+        const bool there = t.there && c * kCols < cache.head_dim;
+        if constexpr (kCols == 4) {
+          v[j][0] = there ? *reinterpret_cast<const uint32_t*>(p) : 0;
+        } else if constexpr (kCols == 8) {
+          u32x2 w = {0, 0};
+          if (there) w = *reinterpret_cast<const u32x2*>(p);
+          v[j][0] = w.x;
+          v[j][1] = w.y;
+        } else {
+          u32x4 w = {0, 0, 0, 0};
+          if (there) w = *reinterpret_cast<const u32x4*>(p);
+          v[j][0] = w.x;
+          v[j][1] = w.y;
+          v[j][2] = w.z;
+          v[j][3] = w.w;
+        }
+      }
+      float ks[2], vs[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ks[t] = tiles[t].there ? cache.k_scale[tiles[t].scale] * a.scale : 0.0f;
+        vs[t] = tiles[t].there ? cache.v_scale[tiles[t].scale] : 0.0f;
+      }
+      // Keys that some row may not see, and codes in their places that are no numbers.
+      const bool partial = key0 + kStep - 1 > least || !t0.there || !t1.there;
+      bool mend = false;
+      if (partial) {
+        uint32_t nan = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int k = 0; k < kCols / 4; ++k) nan |= ((v[j][k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+        mend = __any(nan != 0);
+      }
+      u32x4 p_hi[kTiles], p_lo[kTiles];
+      uint32_t seen[kTiles];  // bit j: this lane's row sees its key j
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        float x[8];
+        seen[n] = 0xFF;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s[n][j / 4][j % 4] * ks[j / 4];
+        if (partial) {
+          seen[n] = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool see = key0 + (j / 4) * 16 + 4 * g + j % 4 <= last[n] && tiles[j / 4].there;
+            x[j] = see ? x[j] : -INFINITY;
+            seen[n] |= see ? 1u << j : 0u;
+          }
+        }
+        float high = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) high = fmaxf(high, x[j]);
+        high = fmaxf(rows_max(high), top[n]);
+        const float base = high == -INFINITY ? 0.0f : high;
+        const float fade = exp2f(top[n] - base);
+        top[n] = high;
+        float p[8], total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = exp2f(x[j] - base);
+          total += p[j];
+        }
+        sum[n] = sum[n] * fade + total;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) o[n][d] *= fade;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float y0 = p[2 * j] * vs[j / 2], y1 = p[2 * j + 1] * vs[j / 2];
+          hi[j] = pack_bf16(y0, y1);
+          if (kParts > 1)
+            lo[j] = pack_bf16(y0 - __uint_as_float(hi[j] << 16), y1 - __uint_as_float(hi[j] & 0xFFFF0000u));
+        }
+        p_hi[n] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+        if (kParts > 1) p_lo[n] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+      }
+      using B = Query<KVX_DTYPE_BF16>;
+#pragma unroll
+      for (int k = 0; k < kCols / 4; ++k) {
+        uint32_t rows_in[8], lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rows_in[j] = v[j][k];
+        transpose4(rows_in, lo);
+        transpose4(rows_in + 4, hi);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          uint32_t l = lo[d], h = hi[d];
+          if (mend) {
+            // A key that is masked for a row adds nothing to it, though its code be NaN: NaN codes
+            // count as zeros, and rows that see one become NaN.
+            const uint32_t l_nan = (((l & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+            const uint32_t h_nan = (((h & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+            l &= ~(l_nan * 0xFFu);
+            h &= ~(h_nan * 0xFFu);
+            const bf16x8 is_nan = decode8<B>(l_nan * 0x38u, h_nan * 0x38u);  // 0x38: 1.0
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+              u32x4 w;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = ((seen[n] >> (2 * j)) & 1u ? 0x3F80u : 0u) | ((seen[n] >> (2 * j + 1)) & 1u ? 0x3F800000u : 0u);
+              const f32x4 hit = B::mfma(is_nan, __builtin_bit_cast(bf16x8, w), f32x4{0, 0, 0, 0});
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[n][4 * k + d][i] += hit[i] > 0.0f ? NAN : 0.0f;
+            }
+          }
+          const bf16x8 w = decode8<B>(l, h);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_hi[n]), o[n][4 * k + d]);
+            if (kParts > 1) o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_lo[n]), o[n][4 * k + d]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) sum[n] = rows_sum(sum[n]);
+
+    // The key waves' parts are joined in LDS, one wave after another adding its own to what is there.
+    if constexpr (kKeyWaves > 1) {
+      __shared__ float joined[kRows][kHd + 4];
+      __shared__ float joined_top[kKeyWaves][kRows], joined_sum[kRows];
+      if (g == 0) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) joined_top[key_wave][n * 16 + c] = top[n];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        float all = joined_top[0][n * 16 + c];
+#pragma unroll
+        for (int w = 1; w < kKeyWaves; ++w) all = fmaxf(all, joined_top[w][n * 16 + c]);
+        const float fade = all == -INFINITY ? 1.0f : exp2f(top[n] - all);
+        top[n] = all;
+        sum[n] *= fade;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) o[n][d] *= fade;
+      }
+      for (int w = 0; w < kKeyWaves; ++w) {
+        if (key_wave == w) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            if (w > 0) sum[n] += joined_sum[n * 16 + c];
+            if (g == 0) joined_sum[n * 16 + c] = sum[n];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float* p = &joined[n * 16 + c][(4 * g + i) * kCols];
+#pragma unroll
+              for (int d = 0; d < kCols; ++d) {
+                if (w > 0) o[n][d][i] += p[d];
+                if (w < kKeyWaves - 1) p[d] = o[n][d][i];
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (key_wave != kKeyWaves - 1) continue;  // the last one holds the whole
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      if (out_row[n] < 0) continue;
+      if (a.splits > 1) {
+        const int64_t total_rows = (int64_t)a.batch.num_tokens * a.q_heads;
+        const int64_t at = split * total_rows + out_row[n];
+        float* dst = a.partial + at * cache.head_dim;
+        float* stats = a.partial + a.splits * total_rows * cache.head_dim + at * 2;
+        if (g == 0) {
+          stats[0] = top[n];
+          stats[1] = sum[n];
+        }
+        if (sum[n] != 0.0f) {  // also for NaN
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int col = (4 * g + i) * kCols;
+            if (col < cache.head_dim) {
+#pragma unroll
+              for (int d = 0; d < kCols; d += 4)
+                *reinterpret_cast<f32x4*>(dst + col + d) = f32x4{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
+            }
+          }
+        }
+        continue;
+      }
+      const float inverse = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+      if (a.lse && g == 0) a.lse[out_row[n]] = (top[n] + log2f(sum[n])) * 0.69314718055994531f;
+      T* dst = (T*)a.out + (int64_t)out_row[n] * cache.head_dim;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = (4 * g + i) * kCols;
+        if (col >= cache.head_dim) continue;
+#pragma unroll
+        for (int d = 0; d < kCols; d += 4) {
+          alignas(8) T y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = (T)(sum[n] == 0.0f ? 0.0f : o[n][d + j][i] * inverse);
+          *reinterpret_cast<u32x2*>(dst + col + d) = *reinterpret_cast<const u32x2*>(y);
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits: a wave per query row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttentionArgs a) {
+  const int lane = threadIdx.x % kWave;
+  const int seq = blockIdx.y;
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int num_rows = rows.count * a.q_heads;
+  const int64_t total_rows = (int64_t)a.batch.num_tokens * a.q_heads;
+  const int hd = a.cache.head_dim;
+  for (int r = blockIdx.x * kWaves + threadIdx.x / kWave; r < num_rows; r += gridDim.x * kWaves) {
+    const int64_t row = (int64_t)rows.first * a.q_heads + r;
+    const float* stats = a.partial + a.splits * total_rows * hd;
+    float top = -INFINITY, sum = 0.0f;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, stats[(s * total_rows + row) * 2]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    f32x4 o = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+      const float part = stats[(s * total_rows + row) * 2 + 1];
+      if (part == 0.0f) continue;
+      const float fade = exp2f(stats[(s * total_rows + row) * 2] - base);
+      sum += part * fade;
+      if (lane * 4 < hd) o += *reinterpret_cast<const f32x4*>(a.partial + (s * total_rows + row) * hd + lane * 4) * fade;
+    }
+    if (a.lse && lane == 0) a.lse[row] = (top + log2f(sum)) * 0.69314718055994531f;
+    if (lane * 4 < hd) {
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      alignas(8) T y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = (T)(o[j] * inverse);
+      *reinterpret_cast<u32x2*>((T*)a.out + row * hd + lane * 4) = *reinterpret_cast<const u32x2*>(y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The weight of each cached token: out = weights + the sum over the query rows
+// of exp(score - lse). A wave holds 32 keys' K and passes over all query rows.
+
+template <int kType, int kHd>
+__global__ __launch_bounds__(kThreads) void weights_kernel(WeightsArgs a) {
+  using Q = Query<kType>;
+  using T = typename Q::T;
+  using Vec = typename Q::Vec;
+  constexpr int kChunks = kHd / 64;
+  const Fp8Cache& cache = a.cache;
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int pairs = a.batch.num_seqs * cache.heads;
+  const int pair = blockIdx.x % pairs;
+  const int seq = pair / cache.heads, head = pair % cache.heads;
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int context = context_of(a.batch, seq, cache.block_size);
+  const int num_rows = rows.count * a.per_kv;
+  const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
+  const int64_t base = (int64_t)pair * a.width;
+  const int key0 = ((blockIdx.x / pairs) * kWaves + wave) * kStep;
+  if (key0 >= a.width) return;
+  float total[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) total[j] = 0.0f;
+  if (key0 < context) {
+    const Tile tiles[2] = {tile_at(cache, table, key0, context, head), tile_at(cache, table, key0 + 16, context, head)};
+    Vec k[2][2 * kChunks];
+    float ks[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* p = cache.k + (tiles[t].row + (int64_t)c * cache.heads) * cache.head_dim;
+      ks[t] = tiles[t].there ? cache.k_scale[tiles[t].scale] * a.scale : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int at = i * 64 + g * 16;
+        u32x4 w = {0, 0, 0, 0};
+        if (tiles[t].there && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(p + at);
+        k[t][2 * i] = decode8<Q>(w.x, w.y);
+        k[t][2 * i + 1] = decode8<Q>(w.z, w.w);
+      }
+    }
+    // Rows before this one see none of the keys.
+    const int first_query = key0 - (context - rows.count);
+    const int first_row = first_query > 0 ? first_query * a.per_kv / 16 * 16 : 0;
+    for (int row0 = first_row; row0 < num_rows; row0 += 16) {
+      const int r = row0 + c;
+      const bool real = r < num_rows;
+      const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
+      const int last = real ? context - rows.count + nth : -1;
+      const int q_head = head * a.per_kv + sub;
+      const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride + (int64_t)q_head * cache.head_dim;
+      const float lse = real ? a.lse[(int64_t)(rows.first + nth) * a.q_heads + q_head] * 1.4426950408889634f : 0.0f;
+      f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int at = i * 64 + g * 16;
+        u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        if (real && at < cache.head_dim) {
+          lo = *reinterpret_cast<const u32x4*>(src + at);
+          hi = *reinterpret_cast<const u32x4*>(src + at + 8);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          s[t] = Q::mfma(k[t][2 * i], __builtin_bit_cast(Vec, lo), s[t]);
+          s[t] = Q::mfma(k[t][2 * i + 1], __builtin_bit_cast(Vec, hi), s[t]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool see = key0 + (j / 4) * 16 + 4 * g + j % 4 <= last && tiles[j / 4].there && lse != -INFINITY;
+        total[j] += see ? exp2f(s[j / 4][j % 4] * ks[j / 4] - lse) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) total[j] += __shfl_xor(total[j], d);
+  }
+  if (c == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = key0 + (j / 4) * 16 + 4 * g + j % 4;
+      if (key < a.width) a.out[base + key] = (a.weights ? a.weights[base + key] : 0.0f) + total[j];
+    }
+  }
+}
+
+int padded_head(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+template <int kType, int kHd, int kTiles, int kRowWaves, int kParts>
+hipError_t attention_of(AttentionArgs a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.batch.max_seqlen * a.per_kv, per = (int64_t)16 * kTiles * kRowWaves;
+  a.row_tiles = (int32_t)((rows + per - 1) / per);
+  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles;
+  attention_kernel<kType, kHd, kTiles, kRowWaves, kParts><<<dim3((unsigned)grid), dim3(kThreads), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+constexpr int kFewRows = 16;
+
+template <int kType, int kHd>
+hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
+  using T = typename Query<kType>::T;
+  constexpr int kManyTiles = kHd == 256 ? 2 : 4;
+  hipError_t err;
+  if ((int64_t)a.batch.max_seqlen * a.per_kv <= kFewRows) err = attention_of<kType, kHd, 1, 1, 2>(a, stream);
+  else err = attention_of<kType, kHd, kManyTiles, 4, kType == KVX_DTYPE_BF16 ? 1 : 2>(a, stream);
+  if (err != hipSuccess || a.splits == 1) return err;
+  const int64_t rows = (int64_t)a.batch.max_seqlen * a.q_heads;
+  const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves), (unsigned)a.batch.num_seqs);
+  join_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <int kType>
+hipError_t attention_sized(const AttentionArgs& a, hipStream_t stream) {
+  switch (padded_head(a.cache.head_dim)) {
+    case 64: return attention_typed<kType, 64>(a, stream);
+    case 128: return attention_typed<kType, 128>(a, stream);
+    default: return attention_typed<kType, 256>(a, stream);
+  }
+}
+
+template <int kType>
+hipError_t weights_sized(const WeightsArgs& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * ((a.width + kWaves * kStep - 1) / (kWaves * kStep));
+  const dim3 g((unsigned)grid), b(kThreads);
+  switch (padded_head(a.cache.head_dim)) {
+    case 64: weights_kernel<kType, 64><<<g, b, 0, stream>>>(a); break;
+    case 128: weights_kernel<kType, 128><<<g, b, 0, stream>>>(a); break;
+    default: weights_kernel<kType, 256><<<g, b, 0, stream>>>(a); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int32_t attention_splits(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads) {
+  const int64_t rows = (int64_t)b.max_seqlen * (q_heads / c.heads);
+  if (rows > kFewRows) return 1;
+  const int64_t groups = (int64_t)b.num_seqs * c.heads;
+  const int64_t steps = ((int64_t)b.table_width * c.block_size + kStep - 1) / kStep;
+  const int64_t want = (1024 + groups - 1) / groups, most = steps / (kWaves * 2);
+  const int64_t n = want < most ? want : most;
+  return n < 1 ? 1 : n > 64 ? 64 : (int32_t)n;
+}
+
+int64_t attention_workspace(int32_t splits, int64_t num_tokens, int32_t q_heads, int32_t head_dim) {
+  return splits <= 1 ? 0 : (int64_t)splits * num_tokens * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+hipError_t launch_attention(AttentionArgs a, int32_t dtype, hipStream_t stream) {
+  return dtype == KVX_DTYPE_BF16 ? attention_sized<KVX_DTYPE_BF16>(a, stream)
+                                 : attention_sized<KVX_DTYPE_FP16>(a, stream);
+}
+
+hipError_t launch_attention_weights(const WeightsArgs& a, int32_t dtype, hipStream_t stream) {
+  return dtype == KVX_DTYPE_BF16 ? weights_sized<KVX_DTYPE_BF16>(a, stream) : weights_sized<KVX_DTYPE_FP16>(a, stream);
+}
+
+}  // namespace kvx

@@ -17,11 +17,12 @@ from pathlib import Path
 import torch  # must precede the dlopen below
 
 LIB_PATH = Path(__file__).resolve().with_name("libkvx.so")
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 E_INVALID, E_RANGE, E_STATE, E_UNSUPPORTED = -1, -2, -3, -4
 SCALE_BF16, SCALE_FP32 = 0, 1
 FORMAT_RAW, FORMAT_FP8 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 DEBUG_SKIP_SAVE_WAIT, DEBUG_SKIP_SLOT_READ_WAIT, DEBUG_SKIP_REUSE_WAIT, DEBUG_SKIP_VICTIM_WAIT = 1, 2, 4, 8
 DEBUG_SKIP_OVERWRITE_WAIT = 16
 NOALLOC_SCRATCH_BYTES = 64 << 20  # KVX_NOALLOC_SCRATCH_BYTES
@@ -49,6 +50,39 @@ class BlockLayout(ctypes.Structure):
         return ("BlockLayout(" + ", ".join(f"{name}={getattr(self, name)}" for name, _ in self._fields_) + ")")
 
 
+class Fp8Cache(ctypes.Structure):
+    """kvx_fp8_cache: a layer's e4m3 codes and the scales of their (group of tokens, KV head)s."""
+
+    _fields_ = [
+        ("k_codes", _c_p),
+        ("v_codes", _c_p),
+        ("k_scales", _c_p),
+        ("v_scales", _c_p),
+        ("num_blocks", _i32),
+        ("block_size", _i32),
+        ("group_size", _i32),
+        ("num_heads", _i32),
+        ("head_dim", _i32),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    """kvx_paged_batch: the sequences of a call, their blocks, lengths and query rows."""
+
+    _fields_ = [
+        ("block_tables", _c_p),
+        ("context_lens", _c_p),
+        ("cu_seqlens", _c_p),
+        ("table_stride", _i64),
+        ("table_width", _i32),
+        ("num_seqs", _i32),
+        ("max_seqlen", _i32),
+        ("num_tokens", _i32),
+    ]
+
+
+_cache_p, _batch_p, _f32 = ctypes.POINTER(Fp8Cache), ctypes.POINTER(PagedBatch), ctypes.c_float
+
 # name -> (restype, argtypes); every function declared in include/kvx.h.
 SIGNATURES = {
     "kvx_entry_layout": (_i32, [ctypes.POINTER(BlockLayout), _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
@@ -66,6 +100,15 @@ SIGNATURES = {
                                      _c_p]),
     "kvx_scatter_tokens_fp8": (_i32, [_c_p, ctypes.POINTER(BlockLayout), ctypes.POINTER(_i32), _i32, _i64, _c_p,
                                       _c_p, _c_p]),
+    "kvx_rotary_embed": (_i32, [_c_p, _i64, _c_p, _i64, _c_p, _i64, _c_p, _i64, _c_p, _i32, _c_p, _i64, _i32, _i32,
+                                _i32, _i32, _i32, _f32, _i32, _c_p]),
+    "kvx_store_kvcache_fp8": (_i32, [_cache_p, _c_p, _i64, _c_p, _i64, _i32, _c_p, _i64, _c_p]),
+    "kvx_attention_fp8_workspace": (_i32, [_cache_p, _batch_p, _i32, ctypes.POINTER(_i64)]),
+    "kvx_attention_fp8": (_i32, [_cache_p, _batch_p, _c_p, _i64, _i32, _i32, _f32, _c_p, _c_p, _c_p, _i64, _c_p]),
+    "kvx_attention_weights_fp8": (_i32, [_cache_p, _batch_p, _c_p, _i64, _i32, _i32, _f32, _c_p, _c_p, _c_p, _i64,
+                                         _c_p]),
+    "kvx_select_tokens": (_i32, [_c_p, _c_p, _i32, _i32, _i64, _i32, _i32, _c_p, _c_p, _c_p, _c_p]),
+    "kvx_compact_kvcache_fp8": (_i32, [_cache_p, _batch_p, _c_p, _c_p, _i32, _c_p, _i64, _i32, _c_p]),
     "kvx_cache_create": (_i32, [_c_p, ctypes.POINTER(BlockLayout), _i32, _c_p, _c_p, _i32, ctypes.POINTER(_c_p)]),
     "kvx_cache_destroy": (_i32, [_c_p]),
     "kvx_cache_set_staging": (_i32, [_c_p, _c_p, _c_p, _i32]),

@@ -9,7 +9,7 @@ torch-op fallback, so a missing or unloadable libkvx raises.
 
 import ctypes
 import threading
-from math import prod
+from math import ceil, floor, log, pi, prod
 
 import numpy as np
 import torch
@@ -315,6 +315,317 @@ def upload(values: np.ndarray, device: torch.device, stream=None, out: torch.Ten
         check(lib().kvx_upload(out.data_ptr(), buf.data_ptr(), host.nbytes, _stream(device, s)), "upload")
         ring.read_by(slot, s)
     return out
+
+
+# ---------------------------------------------------------------------------
+# A serving step around an e4m3 KV cache: rotary positions, the cache write, attention, eviction
+#
+# Such a cache is a float8_e4m3fn pool [2, L, NB, BS, H, hd] and its scales, a float32 pool [2, L, NB, BS / G, H, 1]:
+# one scale for each group of G tokens of a block and each KV head. The operators take a layer's views of both, e.g.
+# pool[0, layer], pool[1, layer], scales[0, layer], scales[1, layer]; save_blocks and restore_blocks (FORMAT_RAW) move
+# the blocks of either pool.
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int | None = None, fast: float = 32.0, slow: float = 1.0,
+                       device=None) -> tuple[torch.Tensor, float]:
+    """(frequencies, magnitude) for rotary_embed: rotary_dim / 2 float64 radians a position, and the outputs' factor.
+
+    Pair i turns by base ** (-2 i / rotary_dim) a position. For contexts `factor` times as long as the trained one:
+    - "linear": all positions are divided by `factor`;
+    - "base": the base grows so that the slowest pair turns `factor` times slower and the fastest as before;
+    - "by_parts": pairs that turn `fast` times or more over original_length positions stay, those that turn `slow`
+      times or less are divided by `factor`, those between are blended linearly in their index, and outputs grow by
+      0.1 ln(factor) + 1.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even (got {rotary_dim})")
+    if base <= 0 or factor < 1:
+        raise ValueError(f"base must be positive and factor at least 1 (got {base} and {factor})")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if scaling not in (None, "linear", "base", "by_parts"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    index = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    frequencies = base ** (-2.0 * index / rotary_dim)
+    magnitude = 1.0
+    if scaling == "linear":
+        frequencies = frequencies / factor
+    elif scaling == "by_parts":
+        if original_length is None or original_length <= 0 or fast <= slow or slow <= 0 or base <= 1:
+            raise ValueError("by_parts needs a positive original_length, fast > slow > 0 and base > 1")
+
+        def pair_turning(times: float) -> float:
+            return rotary_dim * log(original_length / (times * 2 * pi)) / (2 * log(base))
+
+        low, high = max(0, floor(pair_turning(fast))), min(rotary_dim // 2 - 1, ceil(pair_turning(slow)))
+        blend = ((index - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)  # 0: stays, 1: divided
+        frequencies = frequencies * (1 - blend) + frequencies / factor * blend
+        magnitude = 0.1 * log(factor) + 1.0
+    return frequencies.to(device), magnitude
+
+
+def _heads_of(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    if t.ndim != 3 or (t.numel() and (t.stride(2) != 1 or t.stride(1) != t.shape[2])):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with packed heads")
+    return t.shape
+
+
+def rotary_embed(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor,
+                 interleaved: bool = False, magnitude: float = 1.0, query_out: torch.Tensor | None = None,
+                 key_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Queries and keys rotated by their positions: (query_out, key_out), new tensors unless given.
+
+    query, key: [N, heads, head_dim], bfloat16, float16 or float32, with packed heads (the token stride may differ,
+    e.g. views of a fused QKV output). positions: int32 or int64 [N]. frequencies: float64 [rotary_dim / 2], radians
+    a position (rotary_frequencies). The first rotary_dim elements of each head are rotated in pairs
+    (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved, and multiplied by magnitude; the rest is copied. An output
+    may be its input (in place) but may not overlap it otherwise. Angles are taken in float64. Capturable.
+    """
+    n, q_heads, hd = _heads_of(query, "query")
+    kn, k_heads, khd = _heads_of(key, "key")
+    if kn != n or khd != hd:
+        raise ValueError("query and key differ in tokens or head_dim")
+    dtype = query.dtype
+    if dtype not in _DTYPES:
+        raise NotImplementedError(f"rotary_embed takes bfloat16, float16 or float32 tensors, not {dtype}")
+    query_out = torch.empty((n, q_heads, hd), dtype=dtype, device=query.device) if query_out is None else query_out
+    key_out = torch.empty((n, k_heads, hd), dtype=dtype, device=key.device) if key_out is None else key_out
+    if _heads_of(query_out, "query_out") != query.shape or _heads_of(key_out, "key_out") != key.shape:
+        raise ValueError("an output's shape differs from its input's")
+    if not (key.dtype == query_out.dtype == key_out.dtype == dtype):
+        raise TypeError("query, key and their outputs must share one dtype")
+    if positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous() or positions.shape != (n,):
+        raise TypeError("positions must be a contiguous int32 or int64 tensor, one for each token")
+    if frequencies.dtype != torch.float64 or not frequencies.is_contiguous() or frequencies.ndim != 1:
+        raise TypeError("frequencies must be a contiguous float64 vector")
+    device = _require_device(query, key, query_out, key_out, positions, frequencies)
+    check(lib().kvx_rotary_embed(query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
+                                 query_out.data_ptr(), query_out.stride(0), key_out.data_ptr(), key_out.stride(0),
+                                 positions.data_ptr(), positions.element_size(), frequencies.data_ptr(), n, q_heads,
+                                 k_heads, hd, 2 * frequencies.numel(), int(interleaved), magnitude, _DTYPES[dtype],
+                                 _stream(device)), "rotary_embed")
+    return query_out, key_out
+
+
+def _fp8_cache(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch.Tensor | None = None,
+               v_scale: torch.Tensor | None = None) -> _lib.Fp8Cache:
+    """kvx_fp8_cache of a layer's codes [NB, BS, H, hd] and scales [NB, BS / G, H, 1] (v_cache None: keys only)."""
+    nb, bs, heads, hd = k_cache.shape if k_cache.ndim == 4 else (0, 0, 0, 0)
+    groups = k_scale.shape[1] if k_scale.ndim == 4 else 0
+    for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
+        if cache is None:
+            continue
+        if cache.dtype != torch.float8_e4m3fn or cache.shape != (nb, bs, heads, hd) or not cache.is_contiguous():
+            raise ValueError("k_cache and v_cache must be equally sized contiguous float8_e4m3fn "
+                             "[blocks, block_size, heads, head_dim] tensors")
+        if scale.dtype != torch.float32 or scale.shape != (nb, groups, heads, 1) or not scale.is_contiguous():
+            raise ValueError("scales must be contiguous float32 [blocks, groups, heads, 1] tensors")
+    if groups <= 0 or bs % groups:
+        raise ValueError(f"{groups} groups do not divide blocks of {bs} tokens")
+    return _lib.Fp8Cache(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), k_scale.data_ptr(),
+                         0 if v_scale is None else v_scale.data_ptr(), nb, bs, bs // groups, heads, hd)
+
+
+def _paged_batch(block_tables: torch.Tensor, context_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                 max_seqlen: int | None = None, num_tokens: int = 0) -> _lib.PagedBatch:
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or \
+            (block_tables.numel() and block_tables.stride(1) != 1 and block_tables.shape[1] > 1):
+        raise TypeError("block_tables must be an int32 [sequences, blocks] tensor with contiguous rows")
+    seqs, width = block_tables.shape
+    if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) or not context_lens.is_contiguous():
+        raise TypeError("context_lens must be a contiguous int32 tensor, one for each sequence")
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (seqs + 1,) or not cu_seqlens.is_contiguous():
+            raise TypeError("cu_seqlens must be a contiguous int32 tensor of sequences + 1")
+        max_seqlen = num_tokens if max_seqlen is None else max_seqlen
+    else:
+        if max_seqlen not in (None, 1):
+            raise ValueError("without cu_seqlens each sequence has one query row: max_seqlen is 1")
+        max_seqlen = min(1, num_tokens)
+    return _lib.PagedBatch(block_tables.data_ptr(), context_lens.data_ptr(),
+                           0 if cu_seqlens is None else cu_seqlens.data_ptr(), block_tables.stride(0), width, seqs,
+                           max_seqlen, num_tokens)
+
+
+def _present(*tensors):
+    return [t for t in tensors if t is not None]
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor):
+    """store_kvcache into an e4m3 cache with one scale for each (group of tokens, KV head).
+
+    key/value: [N, num_heads, head_dim], bfloat16, float16 or float32, packed heads, rows on 16 bytes (the token
+    stride may differ). k_cache/v_cache: contiguous float8_e4m3fn [blocks, block_size, num_heads, head_dim] layer
+    views, k_scale/v_scale: contiguous float32 [blocks, groups, num_heads, 1]; a group is block_size / groups tokens, a
+    multiple of 16. slot_mapping: int32 [N], -1 and slots outside the cache skip a token; the tokens of one group
+    stand together in it, as those of a sequence do.
+
+    A group's scale becomes the least power of two s with |x| <= 448 s for what the call writes there (s >= 2^-100;
+    infinities saturate, NaN stays NaN). A call that does not write a group's first slot continues it: the scale is
+    the larger of the old and the new one, and rows already there are encoded anew where it grew. One that does starts
+    the group over, whatever it held. Capturable in a HIP graph.
+    """
+    n, heads, hd = _heads_of(key, "key")
+    if _heads_of(value, "value") != key.shape:
+        raise ValueError("key and value shapes differ")
+    if key.dtype not in _DTYPES:
+        raise NotImplementedError(f"store_kvcache_fp8 takes bfloat16, float16 or float32 rows, not {key.dtype}")
+    if value.dtype != key.dtype:
+        raise TypeError("key and value must share one dtype")
+    cache = _fp8_cache(k_cache, k_scale, v_cache, v_scale)
+    if (cache.num_heads, cache.head_dim) != (heads, hd):
+        raise ValueError("rows and cache differ in heads or head_dim")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous():
+        raise TypeError("slot_mapping must be a contiguous int32 tensor, one for each token")
+    device = _require_device(k_cache, key, value, v_cache, k_scale, v_scale, slot_mapping)
+    check(lib().kvx_store_kvcache_fp8(ctypes.byref(cache), key.data_ptr(), key.stride(0), value.data_ptr(),
+                                      value.stride(0), _DTYPES[key.dtype], slot_mapping.data_ptr(), n,
+                                      _stream(device)), "store_kvcache_fp8")
+
+
+def _check_queries(query: torch.Tensor, cache: _lib.Fp8Cache):
+    n, heads, hd = _heads_of(query, "query")
+    if query.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"queries of an e4m3 cache are bfloat16 or float16, not {query.dtype}")
+    if hd != cache.head_dim or heads % max(1, cache.num_heads):
+        raise ValueError("query heads must be a multiple of the cache's, with its head_dim")
+    return n, heads, hd
+
+
+def attention_fp8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                  softmax_scale: float | None = None, cu_seqlens: torch.Tensor | None = None,
+                  max_seqlen: int | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Causal attention of each sequence's last tokens over its e4m3 cache: out, or (out, lse) with return_lse.
+
+    query: [N, q_heads, head_dim], bfloat16 or float16, packed heads, rows on 16 bytes; q_heads a multiple of the
+    cache's heads (grouped heads). Caches and scales as store_kvcache_fp8's, which has written this call's tokens
+    already. block_tables: int32 [B, width]; context_lens: int32 [B], all cached tokens of a sequence; entries past
+    a sequence's blocks are not read, ids outside the pool count as blocks without tokens.
+
+    Decode: N == B, row b is sequence b's newest token. Chunks: cu_seqlens, int32 [B + 1], row range of each sequence
+    (row i of n sees the tokens up to context - n + i) and max_seqlen, the most rows of one (a hint that sizes the
+    launch; default N). Rows of no sequence are left as they are; rows that see no token become 0. out: contiguous
+    [N, q_heads, head_dim] of the query's type; lse: float32 [N, q_heads], log of the sum of exp(scores), -inf for
+    rows that see no token. softmax_scale defaults to head_dim ** -0.5. Capturable in a HIP graph.
+    """
+    cache = _fp8_cache(k_cache, k_scale, v_cache, v_scale)
+    n, heads, hd = _check_queries(query, cache)
+    batch = _paged_batch(block_tables, context_lens, cu_seqlens, max_seqlen, n)
+    if out is None:
+        out = torch.empty((n, heads, hd), dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of the query's shape and dtype")
+    device = _require_device(k_cache, query, out, v_cache, k_scale, v_scale, block_tables, context_lens,
+                             *_present(cu_seqlens))
+    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    need = ctypes.c_int64()
+    check(lib().kvx_attention_fp8_workspace(ctypes.byref(cache), ctypes.byref(batch), heads, ctypes.byref(need)),
+          "attention_fp8")
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    check(lib().kvx_attention_fp8(ctypes.byref(cache), ctypes.byref(batch), query.data_ptr(), query.stride(0), heads,
+                                  _DTYPES[query.dtype], hd ** -0.5 if softmax_scale is None else softmax_scale,
+                                  out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                  None if workspace is None else workspace.data_ptr(), need.value, _stream(device)),
+          "attention_fp8")
+    return (out, lse) if return_lse else out
+
+
+def attention_weights_fp8(query: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
+                          block_tables: torch.Tensor, context_lens: torch.Tensor, softmax_scale: float | None = None,
+                          cu_seqlens: torch.Tensor | None = None, max_seqlen: int | None = None,
+                          weights: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Adds up the attention that each cached token received from a call of attention_fp8: what eviction goes by.
+
+    out[b, h, t] = weights[b, h, t] + the sum of the softmax weights of token t over sequence b's rows and the query
+    heads of KV head h. Arguments as attention_fp8's, with the lse that it returned. weights: contiguous float32
+    [B, heads, width] (None: zeros, with width the tables' tokens); out: likewise, may be weights itself; default
+    weights, in place, or a new tensor where weights is None. Tokens at or past width are dropped, and entries past a
+    sequence's context keep their weights. Deterministic. Capturable in a HIP graph.
+    """
+    cache = _fp8_cache(k_cache, k_scale)
+    n, heads, hd = _check_queries(query, cache)
+    batch = _paged_batch(block_tables, context_lens, cu_seqlens, max_seqlen, n)
+    if lse.dtype != torch.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
+        raise TypeError("lse must be a contiguous float32 [tokens, q_heads] tensor")
+    if out is None:
+        out = weights if weights is not None else torch.empty(
+            (batch.num_seqs, cache.num_heads, batch.table_width * cache.block_size), dtype=torch.float32,
+            device=query.device)
+    for t in _present(weights, out):
+        if t.dtype != torch.float32 or t.ndim != 3 or t.shape[:2] != (batch.num_seqs, cache.num_heads) or \
+                t.shape != out.shape or not t.is_contiguous():
+            raise ValueError("weights and out must be contiguous float32 [sequences, heads, width] tensors")
+    device = _require_device(k_cache, query, lse, k_scale, block_tables, context_lens,
+                             *_present(cu_seqlens, weights, out))
+    check(lib().kvx_attention_weights_fp8(ctypes.byref(cache), ctypes.byref(batch), query.data_ptr(), query.stride(0),
+                                          heads, _DTYPES[query.dtype],
+                                          hd ** -0.5 if softmax_scale is None else softmax_scale, lse.data_ptr(),
+                                          None if weights is None else weights.data_ptr(), out.data_ptr(),
+                                          out.shape[2], _stream(device)), "attention_weights_fp8")
+    return out
+
+
+def select_tokens(weights: torch.Tensor, context_lens: torch.Tensor, keep: int,
+                  recent: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The tokens of each (sequence, KV head) to keep, by their accumulated weight: (indices, counts, kept).
+
+    weights: contiguous float32 [B, heads, width]; context_lens: int32 [B] (lengths beyond width count as width). A
+    context of at most `keep` tokens is kept whole. Of a longer one, the last `recent` (at most keep) are kept and, of
+    the others, the keep - recent with the largest weights: of equal ones the earliest, NaN below all. indices: int32
+    [B, heads, keep], ascending, then -1; counts: int32 [B], the kept tokens of each sequence (its context_lens after
+    compact_kvcache_fp8); kept: float32 [B, heads, keep], their weights, then 0. Capturable in a HIP graph.
+    """
+    if weights.dtype != torch.float32 or weights.ndim != 3 or not weights.is_contiguous():
+        raise TypeError("weights must be a contiguous float32 [sequences, heads, width] tensor")
+    seqs, heads, width = weights.shape
+    if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) or not context_lens.is_contiguous():
+        raise TypeError("context_lens must be a contiguous int32 tensor, one for each sequence")
+    if keep < 0 or recent < 0 or heads == 0:
+        raise ValueError("keep and recent must be non-negative, and heads at least 1")
+    device = _require_device(weights, context_lens)
+    indices = torch.empty((seqs, heads, keep), dtype=torch.int32, device=device)
+    counts = torch.empty((seqs,), dtype=torch.int32, device=device)
+    kept = torch.empty((seqs, heads, keep), dtype=torch.float32, device=device)
+    check(lib().kvx_select_tokens(weights.data_ptr(), context_lens.data_ptr(), seqs, heads, width, keep, recent,
+                                  indices.data_ptr(), counts.data_ptr(), kept.data_ptr(), _stream(device)),
+          "select_tokens")
+    return indices, counts, kept
+
+
+def compact_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                        block_tables: torch.Tensor, indices: torch.Tensor, counts: torch.Tensor,
+                        new_block_tables: torch.Tensor, context_lens: torch.Tensor | None = None):
+    """Moves the kept tokens of each KV head to the front of other blocks: position j of sequence b in the blocks
+    new_block_tables[b] becomes its token indices[b, h, j] in the blocks block_tables[b], for j < counts[b].
+
+    Caches, scales and tables as store_kvcache_fp8's and attention_fp8's; indices and counts as select_tokens gives
+    them (an index that is no token of the sequence gives zeros). New blocks may be no block that a table of the call
+    names as a source, nor be named twice: shared prefixes stay as they are for their other users. Each group written
+    gets the scale that store_kvcache_fp8 would give its values. context_lens: int32 [B], where indices may reach past
+    a sequence (default: the tables' tokens). Capturable in a HIP graph.
+    """
+    cache = _fp8_cache(k_cache, k_scale, v_cache, v_scale)
+    seqs = block_tables.shape[0] if block_tables.ndim == 2 else 0
+    if indices.dtype != torch.int32 or indices.ndim != 3 or indices.shape[:2] != (seqs, cache.num_heads) or \
+            not indices.is_contiguous():
+        raise TypeError("indices must be a contiguous int32 [sequences, heads, keep] tensor")
+    if new_block_tables.ndim != 2 or new_block_tables.shape[0] != seqs:
+        raise ValueError("new_block_tables must have a row for each sequence")
+    lens = counts if context_lens is None else context_lens
+    batch = _paged_batch(block_tables, lens)
+    new = _paged_batch(new_block_tables, counts)
+    if context_lens is None:
+        batch.context_lens = None
+    device = _require_device(k_cache, v_cache, k_scale, v_scale, block_tables, indices, counts, new_block_tables, lens)
+    check(lib().kvx_compact_kvcache_fp8(ctypes.byref(cache), ctypes.byref(batch), indices.data_ptr(),
+                                        counts.data_ptr(), indices.shape[2], new_block_tables.data_ptr(),
+                                        new.table_stride, new.table_width, _stream(device)), "compact_kvcache_fp8")
 
 
 # ---------------------------------------------------------------------------
