@@ -173,7 +173,8 @@ _bind = None
 def load_bind():
     """The native operator binding (kvx/_bind.so, csrc/kvx_bind.cpp), calling the loaded libkvx.
 
-    Each of its functions returns libkvx's status, or None for a call it does not take. Raises ImportError if it is
+    Each of its functions returns libkvx's status, or None for a call it does not take; those that make their outputs
+    return them instead of a status of 0. Raises ImportError if it is
     not built, or was built for another torch, and RuntimeError if it was built for another libkvx."""
     handle = lib()
     module = importlib.import_module("kvx._bind")
@@ -183,7 +184,10 @@ def load_bind():
     if module.TORCH_VERSION != torch.__version__:
         raise ImportError(f"kvx._bind was built for torch {module.TORCH_VERSION}, not {torch.__version__}")
     module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
-        handle.kvx_store_kvcache, handle.kvx_save_blocks, handle.kvx_restore_blocks, handle.kvx_entry_layout)))
+        handle.kvx_store_kvcache, handle.kvx_save_blocks, handle.kvx_restore_blocks, handle.kvx_entry_layout,
+        handle.kvx_rotary_embed, handle.kvx_store_kvcache_fp8, handle.kvx_attention_fp8_workspace,
+        handle.kvx_attention_fp8, handle.kvx_attention_weights_fp8, handle.kvx_select_tokens,
+        handle.kvx_compact_kvcache_fp8)))
     return module
 
 
@@ -194,7 +198,7 @@ class _NoBind:
     def store(*args):
         return None
 
-    codec = blocks = store
+    codec = blocks = rotary = store_fp8 = attention = attention_weights = select = compact = store
 
 
 def bind():

@@ -374,6 +374,13 @@ def _heads_of(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     return t.shape
 
 
+def _made(done, what: str):
+    """What the native binding returned in place of outputs it made: those, or the status that kept it from them."""
+    if type(done) is int:
+        check(done, what)
+    return done
+
+
 def rotary_embed(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor,
                  interleaved: bool = False, magnitude: float = 1.0, query_out: torch.Tensor | None = None,
                  key_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -385,6 +392,9 @@ def rotary_embed(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved, and multiplied by magnitude; the rest is copied. An output
     may be its input (in place) but may not overlap it otherwise. Angles are taken in float64. Capturable.
     """
+    done = _bind().rotary(query, key, positions, frequencies, interleaved, magnitude, query_out, key_out)
+    if done is not None:
+        return _made(done, "rotary_embed")
     n, q_heads, hd = _heads_of(query, "query")
     kn, k_heads, khd = _heads_of(key, "key")
     if kn != n or khd != hd:
@@ -470,6 +480,11 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     the larger of the old and the new one, and rows already there are encoded anew where it grew. One that does starts
     the group over, whatever it held. Capturable in a HIP graph.
     """
+    rc = _bind().store_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    if rc is not None:
+        if rc:
+            check(rc, "store_kvcache_fp8")
+        return
     n, heads, hd = _heads_of(key, "key")
     if _heads_of(value, "value") != key.shape:
         raise ValueError("key and value shapes differ")
@@ -514,6 +529,10 @@ def attention_fp8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     [N, q_heads, head_dim] of the query's type; lse: float32 [N, q_heads], log of the sum of exp(scores), -inf for
     rows that see no token. softmax_scale defaults to head_dim ** -0.5. Capturable in a HIP graph.
     """
+    done = _bind().attention(query, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, softmax_scale,
+                             cu_seqlens, max_seqlen, out, return_lse)
+    if done is not None:
+        return _made(done, "attention_fp8")
     cache = _fp8_cache(k_cache, k_scale, v_cache, v_scale)
     n, heads, hd = _check_queries(query, cache)
     batch = _paged_batch(block_tables, context_lens, cu_seqlens, max_seqlen, n)
@@ -548,6 +567,14 @@ def attention_weights_fp8(query: torch.Tensor, lse: torch.Tensor, k_cache: torch
     weights, in place, or a new tensor where weights is None. Tokens at or past width are dropped, and entries past a
     sequence's context keep their weights. Deterministic. Capturable in a HIP graph.
     """
+    into = weights if out is None else out
+    if into is not None:
+        rc = _bind().attention_weights(query, lse, k_cache, k_scale, block_tables, context_lens, softmax_scale,
+                                       cu_seqlens, max_seqlen, weights, into)
+        if rc is not None:
+            if rc:
+                check(rc, "attention_weights_fp8")
+            return into
     cache = _fp8_cache(k_cache, k_scale)
     n, heads, hd = _check_queries(query, cache)
     batch = _paged_batch(block_tables, context_lens, cu_seqlens, max_seqlen, n)
@@ -581,6 +608,9 @@ def select_tokens(weights: torch.Tensor, context_lens: torch.Tensor, keep: int,
     [B, heads, keep], ascending, then -1; counts: int32 [B], the kept tokens of each sequence (its context_lens after
     compact_kvcache_fp8); kept: float32 [B, heads, keep], their weights, then 0. Capturable in a HIP graph.
     """
+    done = _bind().select(weights, context_lens, keep, recent)
+    if done is not None:
+        return _made(done, "select_tokens")
     if weights.dtype != torch.float32 or weights.ndim != 3 or not weights.is_contiguous():
         raise TypeError("weights must be a contiguous float32 [sequences, heads, width] tensor")
     seqs, heads, width = weights.shape
@@ -610,6 +640,11 @@ def compact_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: t
     gets the scale that store_kvcache_fp8 would give its values. context_lens: int32 [B], where indices may reach past
     a sequence (default: the tables' tokens). Capturable in a HIP graph.
     """
+    rc = _bind().compact(k_cache, v_cache, k_scale, v_scale, block_tables, indices, counts, new_block_tables, context_lens)
+    if rc is not None:
+        if rc:
+            check(rc, "compact_kvcache_fp8")
+        return
     cache = _fp8_cache(k_cache, k_scale, v_cache, v_scale)
     seqs = block_tables.shape[0] if block_tables.ndim == 2 else 0
     if indices.dtype != torch.int32 or indices.ndim != 3 or indices.shape[:2] != (seqs, cache.num_heads) or \

@@ -644,3 +644,34 @@ def test_a_sequence_from_prompt_to_eviction(gpu):
         weights[layer, :, :, :keep] = kept
     table, length = [0, 6], keep
     step(1, torch.tensor([153], device=gpu))
+
+
+def test_calls_give_the_same_with_and_without_the_native_binding(gpu, monkeypatch):
+    from kvx import _lib
+
+    s = Setup(gpu, [70, 5, 130], [20, 5, 7], 2, 3, 64, 32, 16)
+    decode = Setup(gpu, [70, 5, 130], None, 2, 3, 64, 32, 16)
+    where, how = s.batch()
+    k, v = rows(6, 2, 64, torch.bfloat16, 1).to(gpu), rows(6, 2, 64, torch.bfloat16, 2).to(gpu)
+    positions, (frequencies, _) = torch.arange(32, device=gpu), ops.rotary_frequencies(64)
+    results = []
+    for binding in (_lib.load_bind(), _lib._NoBind):
+        monkeypatch.setattr(_lib, "_bind", binding)
+        cache = s.caches()
+        out, lse = ops.attention_fp8(s.q.to(gpu), *cache, *where, return_lse=True, **how)
+        alone = ops.attention_fp8(s.q.to(gpu), *cache, *where, s.scale, cu_seqlens=how["cu_seqlens"])
+        single = ops.attention_fp8(decode.q.to(gpu), *decode.caches(), *decode.batch()[0], out=torch.empty_like(decode.q, device=gpu))
+        weights = ops.attention_weights_fp8(s.q.to(gpu), lse, cache[0], cache[2], *where, **how)
+        ops.attention_weights_fp8(s.q.to(gpu), lse, cache[0], cache[2], *where, s.scale, weights=weights, **how)
+        indices, counts, kept = ops.select_tokens(weights, where[1], 9, 3)
+        ops.store_kvcache_fp8(k, v, *cache, int32([3, 4, 5, -1, 40, 41], gpu))
+        turned = ops.rotary_embed(s.q.to(gpu), s.q[:, :2].to(gpu), positions, frequencies, True, 2.0)
+        inplace = s.q.to(gpu)
+        assert ops.rotary_embed(inplace, inplace[:, :0], positions, frequencies, query_out=inplace)[0] is inplace
+        new = int32([[int(s.tables.max()) + 1] * 1] * 3, gpu)
+        ops.compact_kvcache_fp8(*cache, where[0], indices[:1].repeat(3, 1, 1), counts.clamp_max(0), new, where[1])
+        results.append([out, lse, alone, single, weights, indices, counts, kept, *turned, inplace,
+                        *(c.view(torch.uint8) for c in cache)])
+    for a, b in zip(*results):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+    assert torch.equal(results[0][0], results[0][2])
