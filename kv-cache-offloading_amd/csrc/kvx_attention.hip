@@ -426,6 +426,441 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Chunks of prompts: many query rows, bound by the matrix cores and the
+// softmax's VALU work beside them.
+//
+// A workgroup of four waves takes 4 * 32 * kCols query rows of one (sequence, KV
+// head) and passes over the keys kKeys at a time. The waves convert the codes
+// to bf16 (K: the query's type) into LDS once for all of them: K's rows as they
+// are, V transposed, with the exponent of its scale applied by the converting
+// instruction. LDS is double-buffered, the codes of the next keys are loaded
+// into registers while the present ones are used, and their blocks are looked
+// up one pass before that.
+// As above, S^T = K Q^T and O^T = V^T P^T, now by mfma 32x32x16: lane (n, h), n =
+// lane % 32, h = lane / 32, gets query row n's scores of keys 8 (i / 4) + 4 h + i % 4;
+// V^T's rows in LDS hold the keys in the order in which P lies in the lanes.
+// A wave's step is 32 keys: the scores of the next step, the softmax of this
+// one and the output of the one before it are independent of each other, so that
+// the matrix cores work under the softmax.
+// The maximum that exponents are taken from moves only when a score exceeds it
+// by 2^8: P <= 2^8 costs bf16 and fp32 no precision, and most steps need neither
+// a reduction over lanes nor a pass over the outputs.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int kType>
+__device__ __forceinline__ f32x16 mfma32(typename Query<kType>::Vec a, typename Query<kType>::Vec b, f32x16 c) {
+  if constexpr (kType == KVX_DTYPE_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Two codes as bf16, times 2^exponent of `scale`.
+__device__ __forceinline__ uint32_t pair_scaled(uint32_t codes, float scale, bool high) {
+  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+}
+
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0x80 in each byte that is a NaN code
+  return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
+// What a pass needs to know of its keys' 16-key tiles.
+template <int kTiles16>
+struct KeyInfo {
+  int64_t row[kTiles16];  // slot * heads + head of the first key, or -1
+  float k_scale[kTiles16], v_scale[kTiles16];
+};
+
+template <int kType, int kHd, int kWaves, int kCols, int kKeys, int kParts>
+__global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
+  using Q = Query<kType>;
+  using T = typename Q::T;
+  using Vec = typename Q::Vec;
+  constexpr int kThreads = kWaves * kWave;
+  constexpr int kRows = 32 * kCols;           // of a wave
+  constexpr int kSteps = kKeys / 32;
+  constexpr int kTiles16 = kKeys / 16;
+  constexpr int kDots = kHd / 16;             // mfmas over the head for 32 keys
+  constexpr int kOuts = kHd / 32;             // tiles of 32 output columns
+  constexpr int kKRow = kHd * 2 + 16;         // bytes between rows in LDS: 16 more, so that 8 lanes' pieces meet no bank twice
+  constexpr int kVRow = kKeys * 2 + 16;
+  constexpr int kKLoads = kKeys * kHd / 16 / kThreads;  // 16-byte pieces of K a thread
+  constexpr int kVCols = kWaves == 4 && kHd > 64 ? 8 : 4;  // adjacent columns of V that a thread transposes
+  constexpr int kVThreads = kHd / kVCols;               // for a group of 8 keys
+  constexpr int kVLoads = kKeys / 8 * kVThreads / kThreads;
+  static_assert(kKLoads * kThreads * 16 == kKeys * kHd && kVLoads * kThreads == kKeys / 8 * kVThreads, "whole pieces");
+  __shared__ alignas(16) uint8_t k_lds[2][kKeys * kKRow];
+  __shared__ alignas(16) uint8_t v_lds[2][kHd * kVRow];
+  __shared__ KeyInfo<kTiles16> info[4];
+  __shared__ uint32_t nan_steps[4];           // steps of the pass whose V holds NaN codes, zeros in LDS
+  const Fp8Cache& cache = a.cache;
+  const int tid = threadIdx.x, lane = tid % kWave, n32 = lane % 32, h = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int pairs = a.batch.num_seqs * cache.heads;
+  const int pair = blockIdx.x % pairs, tile = a.row_tiles - 1 - blockIdx.x / pairs;
+  const int seq = pair / cache.heads, head = pair % cache.heads;
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int context = context_of(a.batch, seq, cache.block_size);
+  const int num_rows = rows.count * a.per_kv;
+  const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
+  const int64_t row_bytes = (int64_t)cache.heads * cache.head_dim;
+
+  for (int group_row = tile * kWaves * kRows; group_row < num_rows; group_row += a.row_tiles * kWaves * kRows) {
+    const int first_row = group_row + wave * kRows;
+    const int group_last = min(group_row + kWaves * kRows, num_rows) - 1;
+    const int group_most = context - rows.count + (int)a.per_kv_of(group_last);  // last key that a row of the group sees
+    const int group_least = context - rows.count + (int)a.per_kv_of(group_row);
+    const int passes = group_most < 0 ? 0 : group_most / kKeys + 1;
+    const int wave_last = min(first_row + kRows, num_rows) - 1;
+    const int most = wave_last < first_row ? -1 : context - rows.count + (int)a.per_kv_of(wave_last);
+    const int least = context - rows.count + (int)a.per_kv_of(first_row);
+
+    Vec q[kCols][kDots];
+    int last[kCols], out_row[kCols];
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      const int r = first_row + n * 32 + n32;
+      const bool real = r < num_rows;
+      const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
+      last[n] = real ? context - rows.count + nth : -1;
+      out_row[n] = real ? (rows.first + nth) * a.q_heads + head * a.per_kv + sub : -1;
+      const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride +
+                     (int64_t)(head * a.per_kv + sub) * cache.head_dim;
+#pragma unroll
+      for (int d = 0; d < kDots; ++d) {
+        const int at = d * 16 + h * 8;
+        u32x4 w = {0, 0, 0, 0};
+        if (real && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(src + at);
+        q[n][d] = __builtin_bit_cast(Vec, w);
+      }
+    }
+    f32x16 o[kCols][kOuts];
+    float top[kCols], base[kCols], sum[kCols];
+    u32x4 p[kCols][2], p_low[kCols][2];
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      top[n] = -INFINITY;
+      base[n] = sum[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][d][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) p[n][i] = p_low[n][i] = u32x4{0, 0, 0, 0};
+    }
+
+    auto look_up = [&](int pass) {
+      if (tid == 0) nan_steps[pass & 3] = 0;
+      if (tid < kTiles16) {
+        KeyInfo<kTiles16>& to = info[pass & 3];
+        const int key = pass * kKeys + tid * 16;
+        int64_t row = -1, scale = 0;
+        if (key < context) {
+          const int nth = cache.block_of(key), in = key - nth * cache.block_size;
+          const int id = table[nth];
+          if (id >= 0 && id < cache.num_blocks) {
+            row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
+            scale = ((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head;
+          }
+        }
+        to.row[tid] = row;
+        to.k_scale[tid] = row < 0 ? 0.0f : cache.k_scale[scale] * a.scale;
+        to.v_scale[tid] = row < 0 ? 1.0f : cache.v_scale[scale];
+      }
+    };
+    u32x4 k_raw[kKLoads];
+    uint32_t v_raw[kVLoads][8][kVCols / 4];
+    auto load = [&](int pass) {
+      const KeyInfo<kTiles16>& from = info[pass & 3];
+      constexpr int kPieces = kHd / 16;  // of a key's row
+#pragma unroll
+      for (int i = 0; i < kKLoads; ++i) {
+        const int piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 16;
+        const int64_t row = from.row[key / 16];
+        k_raw[i] = u32x4{0, 0, 0, 0};
+        if (row >= 0 && at < cache.head_dim)
+          k_raw[i] = *reinterpret_cast<const u32x4*>(cache.k + row * cache.head_dim + (key % 16) * row_bytes + at);
+      }
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i) {
+        const int group = (i * kThreads + tid) / kVThreads, at = tid % kVThreads * kVCols;
+        const int64_t row = from.row[group / 2];
+        const bool there = row >= 0 && at < cache.head_dim;
+        const uint8_t* src = cache.v + row * cache.head_dim + (group % 2) * 4 * row_bytes + at;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // keys 4 h + 0..3, then 8 + 4 h + 0..3
+          const uint8_t* from_row = src + (j < 4 ? j : j + 4) * row_bytes;
+          if constexpr (kVCols == 4) {
+            v_raw[i][j][0] = there ? *reinterpret_cast<const uint32_t*>(from_row) : 0;
+          } else {
+            u32x2 w = {0, 0};
+            if (there) w = *reinterpret_cast<const u32x2*>(from_row);
+            v_raw[i][j][0] = w.x;
+            v_raw[i][j][1] = w.y;
+          }
+        }
+      }
+    };
+    auto convert = [&](int pass) {
+      const KeyInfo<kTiles16>& from = info[pass & 3];
+      uint8_t* k_to = k_lds[pass & 1];
+      uint8_t* v_to = v_lds[pass & 1];
+      constexpr int kPieces = kHd / 16;
+#pragma unroll
+      for (int i = 0; i < kKLoads; ++i) {
+        const int piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 32;
+        u32x4* to = reinterpret_cast<u32x4*>(k_to + key * kKRow + at);
+        to[0] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].x, k_raw[i].y));
+        to[1] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].z, k_raw[i].w));
+      }
+      const bool masked = pass * kKeys + kKeys - 1 > group_least;  // some row does not see some key
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i) {
+        const int group = (i * kThreads + tid) / kVThreads, col = tid % kVThreads * kVCols;
+        const float scale = from.v_scale[group / 2];
+        const float rest = scale / __uint_as_float(__float_as_uint(scale) & 0x7F800000u);
+        if (masked) {
+          uint32_t nan = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int k = 0; k < kVCols / 4; ++k) nan |= nan_bytes(v_raw[i][j][k]);
+          if (nan) {
+            atomicOr(&nan_steps[pass & 3], 1u << (group / 4));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int k = 0; k < kVCols / 4; ++k) v_raw[i][j][k] &= ~((nan_bytes(v_raw[i][j][k]) >> 7) * 0xFFu);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kVCols / 4; ++k) {
+          uint32_t in[8], lo[4], hi[4];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) in[j] = v_raw[i][j][k];
+          transpose4(in, lo);
+          transpose4(in + 4, hi);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            u32x4 w = {pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
+                       pair_scaled(hi[d], scale, false), pair_scaled(hi[d], scale, true)};
+            if (rest != 1.0f) {  // no power of two: the rest of the scale costs V one rounding to bf16
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = pack_bf16(__uint_as_float(w[j] << 16) * rest, __uint_as_float(w[j] & 0xFFFF0000u) * rest);
+            }
+            // The XOR spreads neighbouring threads' columns, kVCols rows apart, over the banks.
+            const int row = col + 4 * k + d;
+            *reinterpret_cast<u32x4*>(v_to + row * kVRow + ((group ^ (row / 8 % 8)) * 16)) = w;
+          }
+        }
+      }
+    };
+    // S^T of 32 keys.
+    auto scores = [&](int buffer, int step, f32x16 (&s)[kCols]) {
+      const uint8_t* from = k_lds[buffer] + (step * 32 + n32) * kKRow + h * 16;
+#pragma unroll
+      for (int n = 0; n < kCols; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kDots; ++d) {
+        const Vec k = *reinterpret_cast<const Vec*>(from + d * 32);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) s[n] = mfma32<kType>(k, q[n][d], s[n]);
+      }
+    };
+    // O^T += V^T P^T of 32 keys. With the XOR above, a lane's row d * 32 + n32 holds the 8 keys 4 step + 2 i + h in the
+    // place (step ^ d) % 2 * 4 + (2 i + h ^ n32 / 8) of the 8 that step / 2 begins.
+    const int v_lane[2] = {n32 * kVRow + (h ^ (n32 / 8)) * 16, n32 * kVRow + ((2 + h) ^ (n32 / 8)) * 16};
+    auto add_outputs = [&](int buffer, int step) {
+      const uint8_t* from = v_lds[buffer] + step / 2 * 128;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* even = from + step % 2 * 64 + v_lane[i];
+        const uint8_t* odd = from + (1 - step % 2) * 64 + v_lane[i];
+#pragma unroll
+        for (int d = 0; d < kOuts; ++d) {
+          const bf16x8 v = *reinterpret_cast<const bf16x8*>((d % 2 ? odd : even) + d * 32 * kVRow);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            o[n][d] = mfma32<KVX_DTYPE_BF16>(v, __builtin_bit_cast(bf16x8, p[n][i]), o[n][d]);
+            if (kParts > 1) o[n][d] = mfma32<KVX_DTYPE_BF16>(v, __builtin_bit_cast(bf16x8, p_low[n][i]), o[n][d]);
+          }
+        }
+      }
+    };
+
+    if (passes > 0) {
+      look_up(0);
+      look_up(1);
+      __syncthreads();
+      load(0);
+      convert(0);
+    }
+    __syncthreads();
+    for (int pass = 0; pass < passes; ++pass) {
+      const int buffer = pass & 1;
+      const KeyInfo<kTiles16>& now = info[pass & 3];
+      look_up(pass + 2);
+      if (pass + 1 < passes) load(pass + 1);
+      const int steps = most < pass * kKeys ? 0 : min(kSteps, (most - pass * kKeys) / 32 + 1);
+      if (steps > 0) {
+        f32x16 x[kCols], next[kCols];
+        scores(buffer, 0, x);
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+          {
+            const int key0 = pass * kKeys + step * 32;
+            const float scale[2] = {now.k_scale[step * 2], now.k_scale[step * 2 + 1]};
+            const bool there[2] = {now.row[step * 2] >= 0, now.row[step * 2 + 1] >= 0};
+            if (key0 + 31 > least || !there[0] || !there[1]) {
+#pragma unroll
+              for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const bool see = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last[n] && there[i / 8];
+                  x[n][i] = see ? x[n][i] * scale[i / 8] : -INFINITY;
+                }
+            } else {
+#pragma unroll
+              for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[n][i] *= scale[i / 8];
+            }
+            float high[kCols];
+            bool over = false;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) {
+              high[n] = x[n][0];
+#pragma unroll
+              for (int i = 1; i < 16; ++i) high[n] = fmaxf(high[n], x[n][i]);
+              over = over || high[n] > top[n] + 8.0f;
+            }
+            if (__any(over)) {
+#pragma unroll
+              for (int n = 0; n < kCols; ++n) {
+                top[n] = fmaxf(top[n], fmaxf(high[n], __shfl_xor(high[n], 32)));
+                // A whole number, so that `fade` is a power of two and nothing is rounded.
+                const float now_base = top[n] == -INFINITY ? base[n] : ceilf(top[n]);
+                const float fade = __builtin_amdgcn_exp2f(base[n] - now_base);
+                base[n] = now_base;
+                sum[n] *= fade;
+#pragma unroll
+                for (int d = 0; d < kOuts; ++d) o[n][d] *= fade;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    p[n][i][j] = pack_bf16(__uint_as_float(p[n][i][j] << 16) * fade,
+                                           __uint_as_float(p[n][i][j] & 0xFFFF0000u) * fade);
+                    if (kParts > 1)
+                      p_low[n][i][j] = pack_bf16(__uint_as_float(p_low[n][i][j] << 16) * fade,
+                                                 __uint_as_float(p_low[n][i][j] & 0xFFFF0000u) * fade);
+                  }
+              }
+            }
+            scores(buffer, step + 1 < steps ? step + 1 : step, next);
+            add_outputs(buffer, step > 0 ? step - 1 : 0);
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float e0 = __builtin_amdgcn_exp2f(x[n][2 * i] - base[n]);
+                const float e1 = __builtin_amdgcn_exp2f(x[n][2 * i + 1] - base[n]);
+                sum[n] += e0 + e1;
+                hi[i] = pack_bf16(e0, e1);
+                if (kParts > 1)
+                  lo[i] = pack_bf16(e0 - __uint_as_float(hi[i] << 16), e1 - __uint_as_float(hi[i] & 0xFFFF0000u));
+              }
+              p[n][0] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+              p[n][1] = u32x4{hi[4], hi[5], hi[6], hi[7]};
+              if (kParts > 1) {
+                p_low[n][0] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+                p_low[n][1] = u32x4{lo[4], lo[5], lo[6], lo[7]};
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) x[n] = next[n];
+          }
+        }
+        add_outputs(buffer, steps - 1);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) p[n][0] = p[n][1] = p_low[n][0] = p_low[n][1] = u32x4{0, 0, 0, 0};
+        const uint32_t nan = nan_steps[pass & 3];
+        if (nan) {
+          // Rows that see a NaN code in a pass that is masked for others: its columns become NaN.
+#pragma unroll 1
+          for (int step = 0; step < steps; ++step) {
+            if (!(nan >> step & 1)) continue;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+              const int64_t row = now.row[step * 2 + i];
+              if (row < 0) continue;
+              u32x4 seen[kCols];
+#pragma unroll
+              for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int key = pass * kKeys + step * 32 + i * 16 + 4 * h + (j < 2 ? 2 * j : 4 + 2 * j);
+                  seen[n][j] = (key <= last[n] ? 0x3F80u : 0u) | (key + 1 <= last[n] ? 0x3F800000u : 0u);
+                }
+#pragma unroll
+              for (int d = 0; d < kOuts; ++d) {
+                const int col = d * 32 + n32;
+                u32x4 is_nan = {0, 0, 0, 0};
+                if (col < cache.head_dim) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    const int key = 4 * h + (j < 4 ? j : j + 4);
+                    const uint8_t code = cache.v[row * cache.head_dim + key * row_bytes + col];
+                    is_nan[j / 2] |= (code & 0x7F) == 0x7F ? (j % 2 ? 0x3F800000u : 0x3F80u) : 0u;
+                  }
+                }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n) {
+                  f32x16 hit;
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) hit[j] = 0.0f;
+                  hit = mfma32<KVX_DTYPE_BF16>(__builtin_bit_cast(bf16x8, is_nan), __builtin_bit_cast(bf16x8, seen[n]), hit);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) o[n][d][j] += hit[j] > 0.0f ? NAN : 0.0f;
+                }
+              }
+            }
+          }
+        }
+      }
+      if (pass + 1 < passes) convert(pass + 1);
+      __syncthreads();
+    }
+
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      const float total = sum[n] + __shfl_xor(sum[n], 32);
+      if (out_row[n] < 0) continue;
+      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+      if (a.lse && h == 0) a.lse[out_row[n]] = total == 0.0f ? -INFINITY : (base[n] + log2f(total)) * 0.69314718055994531f;
+      T* dst = (T*)a.out + (int64_t)out_row[n] * cache.head_dim;
+#pragma unroll
+      for (int d = 0; d < kOuts; ++d) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int col = d * 32 + 8 * (i / 4) + 4 * h;
+          if (col >= cache.head_dim) continue;
+          alignas(8) T y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = (T)(total == 0.0f ? 0.0f : o[n][d][i + j] * inverse);
+          *reinterpret_cast<u32x2*>(dst + col) = *reinterpret_cast<const u32x2*>(y);
+        }
+      }
+    }
+    __syncthreads();  // before the next rows' passes write to LDS
+  }
+}
+
 // Joins the splits: a wave per query row.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(AttentionArgs a) {
@@ -560,15 +995,26 @@ hipError_t attention_of(AttentionArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <int kType, int kHd, int kWaves, int kCols, int kKeys, int kParts>
+hipError_t chunk_of(AttentionArgs a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.batch.max_seqlen * a.per_kv, per = kWaves * 32 * kCols;
+  a.row_tiles = (int32_t)((rows + per - 1) / per);
+  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.row_tiles;
+  chunk_kernel<kType, kHd, kWaves, kCols, kKeys, kParts><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
 constexpr int kFewRows = 16;
 
 template <int kType, int kHd>
 hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
   using T = typename Query<kType>::T;
-  constexpr int kManyTiles = kHd == 256 ? 2 : 4;
-  hipError_t err;
-  if ((int64_t)a.batch.max_seqlen * a.per_kv <= kFewRows) err = attention_of<kType, kHd, 1, 1, 2>(a, stream);
-  else err = attention_of<kType, kHd, kManyTiles, 4, kType == KVX_DTYPE_BF16 ? 1 : 2>(a, stream);
+  constexpr int kParts = kType == KVX_DTYPE_BF16 ? 1 : 2;
+  if ((int64_t)a.batch.max_seqlen * a.per_kv > kFewRows) {
+    if constexpr (kHd < 256) return chunk_of<kType, kHd, 8, 1, 16384 / kHd, kParts>(a, stream);
+    else return attention_of<kType, kHd, 2, 4, kParts>(a, stream);
+  }
+  const hipError_t err = attention_of<kType, kHd, 1, 1, 2>(a, stream);
   if (err != hipSuccess || a.splits == 1) return err;
   const int64_t rows = (int64_t)a.batch.max_seqlen * a.q_heads;
   const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves), (unsigned)a.batch.num_seqs);
