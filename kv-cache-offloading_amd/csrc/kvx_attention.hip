@@ -90,70 +90,80 @@ __device__ __forceinline__ void transpose4(const uint32_t* x, uint32_t* out) {
   out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// 16 keys that lie in one block and under one scale: where their rows begin,
-// or nothing where the keys are past the context or their block is no block.
-struct Tile {
-  int64_t row;   // slot * heads + head of the first key
-  int64_t scale; // element of the scales
-  bool there;
-};
-__device__ __forceinline__ Tile tile_at(const Fp8Cache& c, const int32_t* table, int key, int context, int head) {
-  Tile t = {0, 0, false};
-  if (key >= context) return t;
-  const int nth = c.block_of(key), in = key - nth * c.block_size;
-  const int id = __builtin_amdgcn_readfirstlane(table[nth]);
-  if (id < 0 || id >= c.num_blocks) return t;
-  t.row = ((int64_t)id * c.block_size + in) * c.heads + head;
-  t.scale = ((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head;
-  t.there = true;
-  return t;
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0x80 in each byte that is a NaN code
+  return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
 
+// Four columns of a query row's weighted sum `y` over one split's keys, taken relative to 2^base and with the weights'
+// sum: the output where there is one split, else a part of it.
+template <typename T>
+__device__ __forceinline__ void write_rows(const AttentionArgs& a, int split, int64_t row, int col, float base,
+                                           float sum, f32x4 y) {
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.batch.num_tokens * a.q_heads, at = split * rows + row;
+    *reinterpret_cast<f32x4*>(a.partial + at * a.cache.head_dim + col) = y;
+    if (col == 0)
+      *reinterpret_cast<f32x2*>(a.partial + a.splits * rows * a.cache.head_dim + at * 2) = f32x2{base, sum};
+    return;
+  }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  alignas(8) T out[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = (T)(sum == 0.0f ? 0.0f : y[j] * inverse);
+  *reinterpret_cast<u32x2*>((T*)a.out + row * a.cache.head_dim + col) = *reinterpret_cast<const u32x2*>(out);
+  if (a.lse && col == 0) a.lse[row] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * 0.69314718055994531f;
+}
+
+// Few query rows: single tokens, proposed ones, short chunks. Bound by the
+// bytes of the codes; the four waves of a workgroup take its split's steps in
+// turn and join their parts in LDS, and the splits of a context are joined by a
+// second launch. A wave looks up 32 steps' blocks and scales at once, a lane
+// for each 16-key tile, and loads a step's codes while it uses those of the one
+// before.
 // kHd: head_dim rounded up to 64, 128 or 256; the columns past head_dim are
-// zeros. kTiles query tiles of 16 rows a wave; kRowWaves of the workgroup's waves
-// take rows of their own, and the others share those and split the keys.
-template <int kType, int kHd, int kTiles, int kRowWaves, int kParts>
-__global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
+// zeros. kTiles query tiles of 16 rows.
+template <int kType, int kHd, int kTiles>
+__global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_rows_kernel(AttentionArgs a) {
   using Q = Query<kType>;
+  using B = Query<KVX_DTYPE_BF16>;
   using T = typename Q::T;
   using Vec = typename Q::Vec;
-  constexpr int kKeyWaves = kWaves / kRowWaves;
   constexpr int kChunks = kHd / 64;    // 64 columns of K: one 16-byte load a lane
   constexpr int kCols = kHd / 16;      // columns of V a lane loads, transposes and accumulates
   constexpr int kRows = 16 * kTiles;
+  __shared__ float parts[kWaves][16][kHd + 4];
+  __shared__ float part_base[kWaves][kRows], part_sum[kWaves][kRows];
   const Fp8Cache& cache = a.cache;
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int row_wave = wave % kRowWaves, key_wave = wave / kRowWaves;
 
   // Workgroup -> (sequence, KV head), query tile, split. Neighbouring
   // workgroups take different heads, so that an XCD keeps to few of them.
   const int pairs = a.batch.num_seqs * cache.heads;
   const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
-  const int split = rest % a.splits;
-  const int tile = a.row_tiles - 1 - rest / a.splits;  // the longest first
+  const int tile = rest % a.row_tiles, split = rest / a.row_tiles;
   const int seq = pair / cache.heads, head = pair % cache.heads;
-  const QueryRows rows = query_rows(a.batch, seq);
   const int context = context_of(a.batch, seq, cache.block_size);
+  const int first_step = split * a.split_steps;
+  // The first split also writes the rows that see nothing.
+  if (first_step * kStep >= context && split > 0) return;
+  const QueryRows rows = query_rows(a.batch, seq);
   const int num_rows = rows.count * a.per_kv;
   const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
+  const int64_t row_bytes = (int64_t)cache.heads * cache.head_dim;
+  const int32_t k_lane = c * (int32_t)row_bytes + g * 16, v_lane = 4 * g * (int32_t)row_bytes + c * kCols;
 
   // A launch covers max_seqlen queries a sequence; longer ones wrap around.
-  for (int tile_row = (tile * kRowWaves + row_wave) * kRows; ; tile_row += a.row_tiles * kRowWaves * kRows) {
-    // With several row waves there is no barrier below; with one, tile_row is the workgroup's.
-    if (tile_row >= num_rows) break;
+  for (int tile_row = tile * kRows; tile_row < num_rows; tile_row += a.row_tiles * kRows) {
     // Query rows and the last key each may see.
     Vec q[kTiles][2 * kChunks];
-    int last[kTiles], out_row[kTiles];
-    int most = -1;
+    int last[kTiles];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       const int r = tile_row + n * 16 + c;
       const bool real = r < num_rows;
       const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
       last[n] = real ? context - rows.count + nth : -1;
-      out_row[n] = real ? (rows.first + nth) * a.q_heads + head * a.per_kv + sub : -1;
-      most = last[n] > most ? last[n] : most;
       const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride +
                      (int64_t)(head * a.per_kv + sub) * cache.head_dim;
 #pragma unroll
@@ -168,45 +178,107 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
         q[n][2 * k + 1] = __builtin_bit_cast(Vec, hi);
       }
     }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor(most, d));
-    most = __builtin_amdgcn_readfirstlane(most);
-    // Every key up to here is seen by all of the wave's rows.
+    const int tile_last = min(tile_row + kRows, num_rows) - 1;
+    const int most = context - rows.count + (int)a.per_kv_of(tile_last);
+    // Every key up to here is seen by all of the tile's rows.
     const int least = context - rows.count + (int)a.per_kv_of(tile_row);
 
     f32x4 o[kTiles][kCols];
-    float top[kTiles], sum[kTiles];
+    float top[kTiles], base[kTiles], sum[kTiles];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       top[n] = -INFINITY;
-      sum[n] = 0.0f;
+      base[n] = sum[n] = 0.0f;
 #pragma unroll
       for (int d = 0; d < kCols; ++d) o[n][d] = f32x4{0, 0, 0, 0};
     }
+    const int end_step = most < 0 ? 0 : min(first_step + a.split_steps, most / kStep + 1);
+    const int my_first = first_step + wave;
+    const int my_steps = my_first < end_step ? (end_step - my_first + kWaves - 1) / kWaves : 0;
 
-    const int steps = (context + kStep - 1) / kStep;
-    const int per_split = (steps + a.splits - 1) / a.splits;
-    const int first_step = split * per_split;
-    int end_step = min(first_step + per_split, steps);
-    end_step = min(end_step, most / kStep + 1);
-    if (most < 0) end_step = first_step;
-    for (int step = first_step + key_wave; step < end_step; step += kKeyWaves) {
-      const int key0 = step * kStep;
-      const Tile t0 = tile_at(cache, table, key0, context, head);
-      const Tile t1 = tile_at(cache, table, key0 + 16, context, head);
-      const Tile tiles[2] = {t0, t1};
-      // K: lane (c, g) takes columns 16 g .. 16 g + 15 of each 64 of key c's row.
+    struct Codes {
+      u32x4 k[2][kChunks];
+      uint32_t v[8][kCols / 4];
+    };
+    int64_t info_row = -1;  // of tile lane % 2 of the batch's step lane / 2
+    float info_k = 0.0f, info_v = 0.0f;
+    auto look_up = [&](int nth) {
+      const int step = my_first + (nth + lane / 2) * kWaves, key = step * kStep + lane % 2 * 16;
+      info_row = -1;
+      info_k = info_v = 0.0f;
+      if (step < end_step && key < context) {
+        const int block = cache.block_of(key), in = key - block * cache.block_size;
+        const int id = table[block];
+        if (id >= 0 && id < cache.num_blocks) {
+          info_row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
+          const int64_t at = ((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head;
+          info_k = cache.k_scale[at] * a.scale;
+          info_v = cache.v_scale[at];
+        }
+      }
+    };
+    auto row_of = [&](int nth, int t) {
+      const int at = nth % 32 * 2 + t;
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)info_row, at);
+      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(info_row >> 32), at);
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    };
+    auto load = [&](int nth, Codes& to) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int64_t row = row_of(nth, t);
+        // K: lane (c, g) takes columns 16 g .. 16 g + 15 of each 64 of key c's row.
+        const uint8_t* k_from = cache.k + row * cache.head_dim;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          to.k[t][k] = u32x4{0, 0, 0, 0};
+          if (row >= 0 && k * 64 + g * 16 < cache.head_dim)
+            to.k[t][k] = *reinterpret_cast<const u32x4*>(k_from + (k_lane + k * 64));
+        }
+        // V: columns kCols c .. of keys 4 g + i.
+        const uint8_t* v_from = cache.v + row * cache.head_dim;
+        const bool there = row >= 0 && c * kCols < cache.head_dim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* p = v_from + (v_lane + i * (int32_t)row_bytes);
+          uint32_t(&v)[kCols / 4] = to.v[4 * t + i];
+          if constexpr (kCols == 4) {
+            v[0] = there ? *reinterpret_cast<const uint32_t*>(p) : 0;
+          } else if constexpr (kCols == 8) {
+            u32x2 w = {0, 0};
+            if (there) w = *reinterpret_cast<const u32x2*>(p);
+            v[0] = w.x;
+            v[1] = w.y;
+          } else {
+            u32x4 w = {0, 0, 0, 0};
+            if (there) w = *reinterpret_cast<const u32x4*>(p);
+            v[0] = w.x;
+            v[1] = w.y;
+            v[2] = w.z;
+            v[3] = w.w;
+          }
+        }
+      }
+    };
+    auto use = [&](int nth, const Codes& codes) {
+      const int key0 = (my_first + nth * kWaves) * kStep;
+      bool there[2];
+      float ks[2], vs[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int at = nth % 32 * 2 + t;
+        there[t] = row_of(nth, t) >= 0;
+        ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(info_k), at));
+        vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(info_v), at));
+      }
       f32x4 s[kTiles][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) s[n][t] = f32x4{0, 0, 0, 0};
-        const uint8_t* p = cache.k + (tiles[t].row + (int64_t)c * cache.heads) * cache.head_dim;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-          const int at = k * 64 + g * 16;
-          u32x4 w = {0, 0, 0, 0};
-          if (tiles[t].there && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(p + at);
+          const u32x4 w = codes.k[t][k];
           const Vec lo = decode8<Q>(w.x, w.y), hi = decode8<Q>(w.z, w.w);
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
@@ -215,44 +287,15 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
           }
         }
       }
-      // V: lane (c, g) takes columns kCols c .. of keys 4 g + i of both tiles.
-      uint32_t v[8][kCols / 4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const Tile& t = tiles[j / 4];
-        const uint8_t* p = cache.v + (t.row + (int64_t)(4 * g + j % 4) * cache.heads) * cache.head_dim + c * kCols;
-        const bool there = t.there && c * kCols < cache.head_dim;
-        if constexpr (kCols == 4) {
-          v[j][0] = there ? *reinterpret_cast<const uint32_t*>(p) : 0;
-        } else if constexpr (kCols == 8) {
-          u32x2 w = {0, 0};
-          if (there) w = *reinterpret_cast<const u32x2*>(p);
-          v[j][0] = w.x;
-          v[j][1] = w.y;
-        } else {
-          u32x4 w = {0, 0, 0, 0};
-          if (there) w = *reinterpret_cast<const u32x4*>(p);
-          v[j][0] = w.x;
-          v[j][1] = w.y;
-          v[j][2] = w.z;
-          v[j][3] = w.w;
-        }
-      }
-      float ks[2], vs[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ks[t] = tiles[t].there ? cache.k_scale[tiles[t].scale] * a.scale : 0.0f;
-        vs[t] = tiles[t].there ? cache.v_scale[tiles[t].scale] : 0.0f;
-      }
       // Keys that some row may not see, and codes in their places that are no numbers.
-      const bool partial = key0 + kStep - 1 > least || !t0.there || !t1.there;
+      const bool partial = key0 + kStep - 1 > least || !there[0] || !there[1];
       bool mend = false;
       if (partial) {
         uint32_t nan = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int k = 0; k < kCols / 4; ++k) nan |= ((v[j][k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+          for (int k = 0; k < kCols / 4; ++k) nan |= nan_bytes(codes.v[j][k]);
         mend = __any(nan != 0);
       }
       u32x4 p_hi[kTiles], p_lo[kTiles];
@@ -267,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
           seen[n] = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const bool see = key0 + (j / 4) * 16 + 4 * g + j % 4 <= last[n] && tiles[j / 4].there;
+            const bool see = key0 + (j / 4) * 16 + 4 * g + j % 4 <= last[n] && there[j / 4];
             x[j] = see ? x[j] : -INFINITY;
             seen[n] |= see ? 1u << j : 0u;
           }
@@ -275,46 +318,45 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
         float high = x[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) high = fmaxf(high, x[j]);
-        high = fmaxf(rows_max(high), top[n]);
-        const float base = high == -INFINITY ? 0.0f : high;
-        const float fade = exp2f(top[n] - base);
-        top[n] = high;
-        float p[8], total = 0.0f;
+        if (__any(high > top[n] + 8.0f)) {  // see the chunks' kernel
+          top[n] = fmaxf(rows_max(high), top[n]);
+          const float now = top[n] == -INFINITY ? base[n] : ceilf(top[n]);
+          const float fade = __builtin_amdgcn_exp2f(base[n] - now);
+          base[n] = now;
+          sum[n] *= fade;
+#pragma unroll
+          for (int d = 0; d < kCols; ++d) o[n][d] *= fade;
+        }
+        float p[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          p[j] = exp2f(x[j] - base);
-          total += p[j];
+          p[j] = __builtin_amdgcn_exp2f(x[j] - base[n]);
+          sum[n] += p[j];
         }
-        sum[n] = sum[n] * fade + total;
-#pragma unroll
-        for (int d = 0; d < kCols; ++d) o[n][d] *= fade;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float y0 = p[2 * j] * vs[j / 2], y1 = p[2 * j + 1] * vs[j / 2];
           hi[j] = pack_bf16(y0, y1);
-          if (kParts > 1)
-            lo[j] = pack_bf16(y0 - __uint_as_float(hi[j] << 16), y1 - __uint_as_float(hi[j] & 0xFFFF0000u));
+          lo[j] = pack_bf16(y0 - __uint_as_float(hi[j] << 16), y1 - __uint_as_float(hi[j] & 0xFFFF0000u));
         }
         p_hi[n] = u32x4{hi[0], hi[1], hi[2], hi[3]};
-        if (kParts > 1) p_lo[n] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        p_lo[n] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
-      using B = Query<KVX_DTYPE_BF16>;
 #pragma unroll
       for (int k = 0; k < kCols / 4; ++k) {
-        uint32_t rows_in[8], lo[4], hi[4];
+        uint32_t in[8], lo[4], hi[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) rows_in[j] = v[j][k];
-        transpose4(rows_in, lo);
-        transpose4(rows_in + 4, hi);
+        for (int j = 0; j < 8; ++j) in[j] = codes.v[j][k];
+        transpose4(in, lo);
+        transpose4(in + 4, hi);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           uint32_t l = lo[d], h = hi[d];
           if (mend) {
             // A key that is masked for a row adds nothing to it, though its code be NaN: NaN codes
             // count as zeros, and rows that see one become NaN.
-            const uint32_t l_nan = (((l & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
-            const uint32_t h_nan = (((h & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+            const uint32_t l_nan = nan_bytes(l) >> 7, h_nan = nan_bytes(h) >> 7;
             l &= ~(l_nan * 0xFFu);
             h &= ~(h_nan * 0xFFu);
             const bf16x8 is_nan = decode8<B>(l_nan * 0x38u, h_nan * 0x38u);  // 0x38: 1.0
@@ -333,95 +375,61 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
             o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_hi[n]), o[n][4 * k + d]);
-            if (kParts > 1) o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_lo[n]), o[n][4 * k + d]);
+            o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_lo[n]), o[n][4 * k + d]);
           }
         }
       }
-    }
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) sum[n] = rows_sum(sum[n]);
-
-    // The key waves' parts are joined in LDS, one wave after another adding its own to what is there.
-    if constexpr (kKeyWaves > 1) {
-      __shared__ float joined[kRows][kHd + 4];
-      __shared__ float joined_top[kKeyWaves][kRows], joined_sum[kRows];
-      if (g == 0) {
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) joined_top[key_wave][n * 16 + c] = top[n];
+    };
+    Codes now, next;
+    for (int nth = 0; nth < my_steps; ++nth) {
+      if (nth % 32 == 0) {  // a new batch of steps
+        look_up(nth);
+        load(nth, now);
       }
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        float all = joined_top[0][n * 16 + c];
-#pragma unroll
-        for (int w = 1; w < kKeyWaves; ++w) all = fmaxf(all, joined_top[w][n * 16 + c]);
-        const float fade = all == -INFINITY ? 1.0f : exp2f(top[n] - all);
-        top[n] = all;
-        sum[n] *= fade;
-#pragma unroll
-        for (int d = 0; d < kCols; ++d) o[n][d] *= fade;
-      }
-      for (int w = 0; w < kKeyWaves; ++w) {
-        if (key_wave == w) {
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
-            if (w > 0) sum[n] += joined_sum[n * 16 + c];
-            if (g == 0) joined_sum[n * 16 + c] = sum[n];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float* p = &joined[n * 16 + c][(4 * g + i) * kCols];
-#pragma unroll
-              for (int d = 0; d < kCols; ++d) {
-                if (w > 0) o[n][d][i] += p[d];
-                if (w < kKeyWaves - 1) p[d] = o[n][d][i];
-              }
-            }
-          }
-        }
-        __syncthreads();
-      }
-      if (key_wave != kKeyWaves - 1) continue;  // the last one holds the whole
+      const bool more = nth + 1 < my_steps && (nth + 1) % 32;
+      if (more) load(nth + 1, next);
+      use(nth, now);
+      if (more) now = next;
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      if (out_row[n] < 0) continue;
-      if (a.splits > 1) {
-        const int64_t total_rows = (int64_t)a.batch.num_tokens * a.q_heads;
-        const int64_t at = split * total_rows + out_row[n];
-        float* dst = a.partial + at * cache.head_dim;
-        float* stats = a.partial + a.splits * total_rows * cache.head_dim + at * 2;
-        if (g == 0) {
-          stats[0] = top[n];
-          stats[1] = sum[n];
-        }
-        if (sum[n] != 0.0f) {  // also for NaN
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = (4 * g + i) * kCols;
-            if (col < cache.head_dim) {
-#pragma unroll
-              for (int d = 0; d < kCols; d += 4)
-                *reinterpret_cast<f32x4*>(dst + col + d) = f32x4{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
-            }
-          }
-        }
-        continue;
+      sum[n] = rows_sum(sum[n]);
+      if (g == 0) {
+        part_base[wave][n * 16 + c] = top[n] == -INFINITY ? -INFINITY : base[n];
+        part_sum[wave][n * 16 + c] = sum[n];
       }
-      const float inverse = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
-      if (a.lse && g == 0) a.lse[out_row[n]] = (top[n] + log2f(sum[n])) * 0.69314718055994531f;
-      T* dst = (T*)a.out + (int64_t)out_row[n] * cache.head_dim;
+    }
+    // The waves' parts, 16 rows at a time; threads take 4 columns of a row.
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = (4 * g + i) * kCols;
-        if (col >= cache.head_dim) continue;
+    for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-        for (int d = 0; d < kCols; d += 4) {
-          alignas(8) T y[4];
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = (T)(sum[n] == 0.0f ? 0.0f : o[n][d + j][i] * inverse);
-          *reinterpret_cast<u32x2*>(dst + col + d) = *reinterpret_cast<const u32x2*>(y);
+        for (int d = 0; d < kCols; d += 4)
+          *reinterpret_cast<f32x4*>(&parts[wave][c][(4 * g + i) * kCols + d]) =
+              f32x4{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
+      __syncthreads();
+#pragma unroll
+      for (int piece = threadIdx.x; piece < 16 * kHd / 4; piece += kThreads) {
+        const int row = piece / (kHd / 4), col = piece % (kHd / 4) * 4, r = tile_row + n * 16 + row;
+        if (r >= num_rows || col >= cache.head_dim) continue;
+        float all = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) all = fmaxf(all, part_base[w][n * 16 + row]);
+        f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float fade = __builtin_amdgcn_exp2f(part_base[w][n * 16 + row] - all);
+          const float part = part_sum[w][n * 16 + row];
+          if (part == 0.0f) continue;  // also where nothing was seen, and `all` is no number to compare with
+          total += part * fade;
+          y += *reinterpret_cast<const f32x4*>(&parts[w][row][col]) * fade;
         }
+        const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
+        const int64_t out_row = (int64_t)(rows.first + nth) * a.q_heads + head * a.per_kv + sub;
+        write_rows<T>(a, split, out_row, col, all, total, y);
       }
+      __syncthreads();
     }
   }
 }
@@ -461,10 +469,6 @@ __device__ __forceinline__ uint32_t pair_scaled(uint32_t codes, float scale, boo
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
 }
 
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0x80 in each byte that is a NaN code
-  return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-}
-
 // What a pass needs to know of its keys' 16-key tiles.
 template <int kTiles16>
 struct KeyInfo {
@@ -498,10 +502,13 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
   const int tid = threadIdx.x, lane = tid % kWave, n32 = lane % 32, h = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int pairs = a.batch.num_seqs * cache.heads;
-  const int pair = blockIdx.x % pairs, tile = a.row_tiles - 1 - blockIdx.x / pairs;
+  const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+  const int tile = a.row_tiles - 1 - rest % a.row_tiles, split = rest / a.row_tiles;  // the longest first
   const int seq = pair / cache.heads, head = pair % cache.heads;
-  const QueryRows rows = query_rows(a.batch, seq);
   const int context = context_of(a.batch, seq, cache.block_size);
+  const int split_passes = a.split_steps * kStep / kKeys, first_pass = split * split_passes;
+  if (first_pass * kKeys >= context && split > 0) return;  // the first split also writes the rows that see nothing
+  const QueryRows rows = query_rows(a.batch, seq);
   const int num_rows = rows.count * a.per_kv;
   const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
   const int64_t row_bytes = (int64_t)cache.heads * cache.head_dim;
@@ -511,7 +518,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     const int group_last = min(group_row + kWaves * kRows, num_rows) - 1;
     const int group_most = context - rows.count + (int)a.per_kv_of(group_last);  // last key that a row of the group sees
     const int group_least = context - rows.count + (int)a.per_kv_of(group_row);
-    const int passes = group_most < 0 ? 0 : group_most / kKeys + 1;
+    const int passes = group_most < 0 ? first_pass : min(first_pass + split_passes, group_most / kKeys + 1);
     const int wave_last = min(first_row + kRows, num_rows) - 1;
     const int most = wave_last < first_row ? -1 : context - rows.count + (int)a.per_kv_of(wave_last);
     const int least = context - rows.count + (int)a.per_kv_of(first_row);
@@ -692,15 +699,15 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       }
     };
 
-    if (passes > 0) {
-      look_up(0);
-      look_up(1);
+    if (passes > first_pass) {
+      look_up(first_pass);
+      look_up(first_pass + 1);
       __syncthreads();
-      load(0);
-      convert(0);
+      load(first_pass);
+      convert(first_pass);
     }
     __syncthreads();
-    for (int pass = 0; pass < passes; ++pass) {
+    for (int pass = first_pass; pass < passes; ++pass) {
       const int buffer = pass & 1;
       const KeyInfo<kTiles16>& now = info[pass & 3];
       look_up(pass + 2);
@@ -841,63 +848,99 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     for (int n = 0; n < kCols; ++n) {
       const float total = sum[n] + __shfl_xor(sum[n], 32);
       if (out_row[n] < 0) continue;
-      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      if (a.lse && h == 0) a.lse[out_row[n]] = total == 0.0f ? -INFINITY : (base[n] + log2f(total)) * 0.69314718055994531f;
-      T* dst = (T*)a.out + (int64_t)out_row[n] * cache.head_dim;
 #pragma unroll
-      for (int d = 0; d < kOuts; ++d) {
+      for (int d = 0; d < kOuts; ++d)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const int col = d * 32 + 8 * (i / 4) + 4 * h;
-          if (col >= cache.head_dim) continue;
-          alignas(8) T y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = (T)(total == 0.0f ? 0.0f : o[n][d][i + j] * inverse);
-          *reinterpret_cast<u32x2*>(dst + col) = *reinterpret_cast<const u32x2*>(y);
+          if (col < cache.head_dim)
+            write_rows<T>(a, split, out_row[n], col, top[n] == -INFINITY ? -INFINITY : base[n], total,
+                          f32x4{o[n][d][i], o[n][d][i + 1], o[n][d][i + 2], o[n][d][i + 3]});
         }
-      }
     }
     __syncthreads();  // before the next rows' passes write to LDS
   }
 }
 
-// Joins the splits: a wave per query row.
+// Joins the splits: a workgroup per query row, its threads over 4 columns of one split after another.
+constexpr int kMaxSplits = 128;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(AttentionArgs a) {
-  const int lane = threadIdx.x % kWave;
-  const int seq = blockIdx.y;
+  __shared__ float fades[kMaxSplits];
+  __shared__ float wave_top[kWaves], wave_sum[kWaves];
+  __shared__ f32x4 parts[kThreads];
+  const int tid = threadIdx.x, seq = blockIdx.y, hd = a.cache.head_dim;
   const QueryRows rows = query_rows(a.batch, seq);
-  const int num_rows = rows.count * a.q_heads;
+  const int context = context_of(a.batch, seq, a.cache.block_size);
+  const int steps = (context + kStep - 1) / kStep, used = steps <= a.split_steps ? 1 : (steps - 1) / a.split_steps + 1;
   const int64_t total_rows = (int64_t)a.batch.num_tokens * a.q_heads;
-  const int hd = a.cache.head_dim;
-  for (int r = blockIdx.x * kWaves + threadIdx.x / kWave; r < num_rows; r += gridDim.x * kWaves) {
+  const float* stats = a.partial + a.splits * total_rows * hd;
+  const int columns = hd <= 64 ? 16 : hd <= 128 ? 32 : 64, groups = kThreads / columns;  // threads of 4 columns
+  const int col = tid % columns * 4, group = tid / columns;
+  for (int r = blockIdx.x; r < rows.count * a.q_heads; r += gridDim.x) {
     const int64_t row = (int64_t)rows.first * a.q_heads + r;
-    const float* stats = a.partial + a.splits * total_rows * hd;
-    float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, stats[(s * total_rows + row) * 2]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-      const float part = stats[(s * total_rows + row) * 2 + 1];
-      if (part == 0.0f) continue;
-      const float fade = exp2f(stats[(s * total_rows + row) * 2] - base);
-      sum += part * fade;
-      if (lane * 4 < hd) o += *reinterpret_cast<const f32x4*>(a.partial + (s * total_rows + row) * hd + lane * 4) * fade;
-    }
-    if (a.lse && lane == 0) a.lse[row] = (top + log2f(sum)) * 0.69314718055994531f;
-    if (lane * 4 < hd) {
-      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-      alignas(8) T y[4];
+    f32x2 mine = {-INFINITY, 0.0f};
+    if (tid < used) mine = *reinterpret_cast<const f32x2*>(stats + (tid * total_rows + row) * 2);
+    float top = mine.x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = (T)(o[j] * inverse);
-      *reinterpret_cast<u32x2*>((T*)a.out + row * hd + lane * 4) = *reinterpret_cast<const u32x2*>(y);
+    for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (tid % kWave == 0) wave_top[tid / kWave] = top;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_top[w]);
+    const float fade = mine.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mine.x - top);
+    float sum = mine.y == 0.0f ? 0.0f : mine.y * fade;
+    if (tid < used) fades[tid] = fade;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+    if (tid % kWave == 0) wave_sum[tid / kWave] = sum;
+    __syncthreads();
+    sum = 0.0f;
+    for (int w = 0; w < kWaves; ++w) sum += wave_sum[w];
+    f32x4 y = {0, 0, 0, 0};
+    if (col < hd) {
+#pragma unroll 4
+      for (int s = group; s < used; s += groups) {
+        const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial + (s * total_rows + row) * hd + col);
+        if (fades[s] != 0.0f) y += part * fades[s];
+      }
     }
+    parts[tid] = y;
+    __syncthreads();
+    if (group == 0 && col < hd) {
+      for (int i = 1; i < groups; ++i) y += parts[i * columns + tid];
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      alignas(8) T out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = (T)(sum == 0.0f ? 0.0f : y[j] * inverse);
+      *reinterpret_cast<u32x2*>((T*)a.out + row * hd + col) = *reinterpret_cast<const u32x2*>(out);
+      if (a.lse && col == 0) a.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // The weight of each cached token: out = weights + the sum over the query rows
 // of exp(score - lse). A wave holds 32 keys' K and passes over all query rows.
+
+// 16 keys that lie in one block and under one scale: where their rows begin,
+// or nothing where the keys are past the context or their block is no block.
+struct Tile {
+  int64_t row;   // slot * heads + head of the first key
+  int64_t scale; // element of the scales
+  bool there;
+};
+__device__ __forceinline__ Tile tile_at(const Fp8Cache& c, const int32_t* table, int key, int context, int head) {
+  Tile t = {0, 0, false};
+  if (key >= context) return t;
+  const int nth = c.block_of(key), in = key - nth * c.block_size;
+  const int id = __builtin_amdgcn_readfirstlane(table[nth]);
+  if (id < 0 || id >= c.num_blocks) return t;
+  t.row = ((int64_t)id * c.block_size + in) * c.heads + head;
+  t.scale = ((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head;
+  t.there = true;
+  return t;
+}
 
 template <int kType, int kHd>
 __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsArgs a) {
@@ -986,38 +1029,41 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsArgs a) {
 
 int padded_head(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-template <int kType, int kHd, int kTiles, int kRowWaves, int kParts>
-hipError_t attention_of(AttentionArgs a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.batch.max_seqlen * a.per_kv, per = (int64_t)16 * kTiles * kRowWaves;
-  a.row_tiles = (int32_t)((rows + per - 1) / per);
+constexpr int kFewRows = 32;  // query rows of one (sequence, KV head) up to which the few-rows kernel runs
+int few_tiles(int64_t rows, int padded) { return rows <= 16 || padded == 256 ? 1 : 2; }
+constexpr int kChunkWaves = 8;
+constexpr int chunk_keys(int padded) { return 16384 / padded; }
+
+template <int kType, int kHd, int kTiles>
+hipError_t few_rows_of(const AttentionArgs& a, hipStream_t stream) {
   const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles;
-  attention_kernel<kType, kHd, kTiles, kRowWaves, kParts><<<dim3((unsigned)grid), dim3(kThreads), 0, stream>>>(a);
+  few_rows_kernel<kType, kHd, kTiles><<<dim3((unsigned)grid), dim3(kThreads), 0, stream>>>(a);
   return hipGetLastError();
 }
-
-template <int kType, int kHd, int kWaves, int kCols, int kKeys, int kParts>
-hipError_t chunk_of(AttentionArgs a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.batch.max_seqlen * a.per_kv, per = kWaves * 32 * kCols;
-  a.row_tiles = (int32_t)((rows + per - 1) / per);
-  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.row_tiles;
-  chunk_kernel<kType, kHd, kWaves, kCols, kKeys, kParts><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
-  return hipGetLastError();
-}
-
-constexpr int kFewRows = 16;
 
 template <int kType, int kHd>
 hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
   using T = typename Query<kType>::T;
-  constexpr int kParts = kType == KVX_DTYPE_BF16 ? 1 : 2;
-  if ((int64_t)a.batch.max_seqlen * a.per_kv > kFewRows) {
-    if constexpr (kHd < 256) return chunk_of<kType, kHd, 8, 1, 16384 / kHd, kParts>(a, stream);
-    else return attention_of<kType, kHd, 2, 4, kParts>(a, stream);
+  const int64_t rows = (int64_t)a.batch.max_seqlen * a.per_kv;
+  hipError_t err;
+  bool few = rows <= kFewRows;
+  if constexpr (kHd == 256) few = true;
+  if (few) {
+    if (few_tiles(rows, kHd) == 1) err = few_rows_of<kType, kHd, 1>(a, stream);
+    else if constexpr (kHd < 256) err = few_rows_of<kType, kHd, 2>(a, stream);
+    else err = hipErrorInvalidValue;
+  } else {
+    if constexpr (kHd < 256) {
+      const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles;
+      chunk_kernel<kType, kHd, kChunkWaves, 1, chunk_keys(kHd), kType == KVX_DTYPE_BF16 ? 1 : 2>
+          <<<dim3((unsigned)grid), dim3(kChunkWaves * kWave), 0, stream>>>(a);
+      err = hipGetLastError();
+    } else {
+      err = hipErrorInvalidValue;
+    }
   }
-  const hipError_t err = attention_of<kType, kHd, 1, 1, 2>(a, stream);
   if (err != hipSuccess || a.splits == 1) return err;
-  const int64_t rows = (int64_t)a.batch.max_seqlen * a.q_heads;
-  const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves), (unsigned)a.batch.num_seqs);
+  const dim3 grid((unsigned)((int64_t)a.batch.max_seqlen * a.q_heads), (unsigned)a.batch.num_seqs);
   join_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(a);
   return hipGetLastError();
 }
@@ -1045,21 +1091,32 @@ hipError_t weights_sized(const WeightsArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int32_t attention_splits(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads) {
+AttentionPlan attention_plan(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads) {
   const int64_t rows = (int64_t)b.max_seqlen * (q_heads / c.heads);
-  if (rows > kFewRows) return 1;
-  const int64_t groups = (int64_t)b.num_seqs * c.heads;
+  const bool few = rows <= kFewRows || padded_head(c.head_dim) == 256;
+  const int64_t tile_rows = few ? 16 * few_tiles(rows, padded_head(c.head_dim)) : 32 * kChunkWaves;
+  AttentionPlan plan;
+  plan.row_tiles = (int32_t)((rows + tile_rows - 1) / tile_rows);
+  const int64_t groups = (int64_t)b.num_seqs * c.heads * plan.row_tiles;
   const int64_t steps = ((int64_t)b.table_width * c.block_size + kStep - 1) / kStep;
-  const int64_t want = (1024 + groups - 1) / groups, most = steps / (kWaves * 2);
-  const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : n > 64 ? 64 : (int32_t)n;
+  // Split while there are too few workgroups to fill the chip, and each keeps enough keys.
+  const int64_t want = few ? 4096 : 512, unit = few ? 8 : chunk_keys(padded_head(c.head_dim)) / kStep, least = few ? 8 : 32;
+  int64_t splits = want / groups;
+  if (splits > steps / least) splits = steps / least;
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  int64_t per = (steps + splits - 1) / splits;
+  per = (per + unit - 1) / unit * unit;
+  if (per < unit) per = unit;
+  plan.split_steps = (int32_t)per;
+  plan.splits = steps == 0 ? 1 : (int32_t)((steps + per - 1) / per);
+  return plan;
 }
 
 int64_t attention_workspace(int32_t splits, int64_t num_tokens, int32_t q_heads, int32_t head_dim) {
   return splits <= 1 ? 0 : (int64_t)splits * num_tokens * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
-hipError_t launch_attention(AttentionArgs a, int32_t dtype, hipStream_t stream) {
+hipError_t launch_attention(const AttentionArgs& a, int32_t dtype, hipStream_t stream) {
   return dtype == KVX_DTYPE_BF16 ? attention_sized<KVX_DTYPE_BF16>(a, stream)
                                  : attention_sized<KVX_DTYPE_FP16>(a, stream);
 }

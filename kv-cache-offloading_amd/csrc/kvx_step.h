@@ -64,8 +64,13 @@ struct AttentionArgs {
   void* out;
   float* lse;       // may be NULL
   float* partial;   // workspace (splits > 1): [splits][num_tokens * q_heads][head_dim], then the maxima and sums
-  int32_t splits;
-  int32_t row_tiles;
+  int32_t splits, split_steps;  // of the keys, and steps of 32 keys of each
+  int32_t row_tiles;            // a launch's, of a sequence's query rows
+};
+
+// How a call is cut into workgroups, by its sizes alone.
+struct AttentionPlan {
+  int32_t splits, split_steps, row_tiles;
 };
 
 struct WeightsArgs {
@@ -86,10 +91,10 @@ hipError_t launch_rotary(const RotaryArgs& a, int32_t dtype, hipStream_t stream)
 hipError_t launch_store_fp8(const Fp8Cache& c, const void* key, int64_t key_stride, const void* value,
                             int64_t value_stride, int32_t dtype, const int32_t* slots, int32_t num_tokens,
                             hipStream_t stream);
-// Splits of the keys that launch_attention uses, and the workspace bytes they need (0 for one).
-int32_t attention_splits(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads);
+// What launch_attention takes in its arguments, and the workspace bytes that so many splits need (0 for one).
+AttentionPlan attention_plan(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads);
 int64_t attention_workspace(int32_t splits, int64_t num_tokens, int32_t q_heads, int32_t head_dim);
-hipError_t launch_attention(AttentionArgs a, int32_t dtype, hipStream_t stream);
+hipError_t launch_attention(const AttentionArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t launch_attention_weights(const WeightsArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t launch_select(const float* weights, int32_t rows, int32_t heads, int32_t width, const int32_t* context_lens,
                          int32_t keep, int32_t recent, int32_t* indices, int32_t* counts, float* kept,

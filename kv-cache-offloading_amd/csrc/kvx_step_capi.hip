@@ -188,7 +188,7 @@ int kvx_attention_fp8_workspace(const kvx_fp8_cache* cache, const kvx_paged_batc
     return set_error(KVX_E_INVALID, "%d query heads are not a multiple of %d KV heads", query_heads, c.heads);
   *bytes = b.num_seqs == 0 || b.num_tokens == 0
                ? 0
-               : attention_workspace(attention_splits(c, b, query_heads), b.num_tokens, query_heads, c.head_dim);
+               : attention_workspace(attention_plan(c, b, query_heads).splits, b.num_tokens, query_heads, c.head_dim);
   return KVX_OK;
 }
 
@@ -211,14 +211,17 @@ int kvx_attention_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, 
   a.scale = softmax_scale * 1.4426950408889634f;
   a.out = out;
   a.lse = lse;
-  a.splits = attention_splits(a.cache, a.batch, query_heads);
+  const AttentionPlan plan = attention_plan(a.cache, a.batch, query_heads);
+  a.splits = plan.splits;
+  a.split_steps = plan.split_steps;
+  a.row_tiles = plan.row_tiles;
   const int64_t need = attention_workspace(a.splits, a.batch.num_tokens, query_heads, a.cache.head_dim);
   if (need > workspace_bytes || (need > 0 && (!workspace || (uintptr_t)workspace % 16)))
     return set_error(KVX_E_INVALID, "attention needs %lld bytes of workspace on 16 bytes (got %lld)", (long long)need,
                      (long long)workspace_bytes);
   a.partial = (float*)workspace;
-  if ((int64_t)a.batch.num_seqs * a.cache.heads * a.splits *
-          (((int64_t)a.batch.max_seqlen * a.per_kv + 15) / 16) > kMostGrid)
+  if ((int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles > kMostGrid / 2 ||
+      (int64_t)a.batch.max_seqlen * query_heads > kMostGrid)
     return set_error(KVX_E_UNSUPPORTED, "too many sequences, heads and queries for one launch");
   return hip_status(launch_attention(a, dtype, (hipStream_t)stream), "attention_fp8 launch");
 }
