@@ -153,110 +153,152 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // the group's scale, under which their rows are encoded. A group that the call
 // enters behind its first slot keeps its rows and the larger of both scales;
 // where that grew, the rows that the call does not write are encoded anew.
+// Rows are read once: a thread keeps its pieces of 8 elements of up to kHold
+// rows in registers from the maximum to the encoding.
+//
+// Which tokens begin a group is known on the device only. A workgroup looks at
+// `chunk` tokens and takes the groups that begin among them one after another.
+
+template <typename T>
+struct Eight {  // elements, as loaded
+  u32x4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void expand(const Eight<T>& e, float* out) {
+  const T* x = reinterpret_cast<const T*>(e.w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) out[j] = (float)x[j];
+}
+__device__ __forceinline__ u32x2 encode8(const float* x, float times) {
+  u32x2 out;
+  out.x = encode4(x[0] * times, x[1] * times, x[2] * times, x[3] * times);
+  out.y = encode4(x[4] * times, x[5] * times, x[6] * times, x[7] * times);
+  return out;
+}
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T* __restrict__ key, int64_t key_stride,
                                                              const T* __restrict__ value, int64_t value_stride,
-                                                             const int32_t* __restrict__ slots, int32_t num_tokens) {
+                                                             const int32_t* __restrict__ slots, int32_t num_tokens,
+                                                             int32_t chunk, int32_t lane_bits) {
+  constexpr int kHold = 4;
   __shared__ int owner[kMaxGroup];  // the call's token for each of the group's rows; the last one that names it
-  __shared__ int run_end;
+  __shared__ int wave_end[kThreads / kWave];
   __shared__ float wave_amax[kThreads / kWave];
-  const int token0 = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int head = blockIdx.y % c.heads;
   const bool is_v = blockIdx.y >= c.heads;
   const int64_t cache_slots = (int64_t)c.num_blocks * c.block_size;
-  const int slot0 = slots[token0];
-  if (slot0 < 0 || slot0 >= cache_slots) return;
-  const int group = c.group_of(slot0);
-  if (token0 > 0) {
-    const int before = slots[token0 - 1];
-    if (before >= 0 && c.group_of(before) == group) return;  // the group's run began earlier
-  }
-  for (int i = threadIdx.x; i < c.group; i += kThreads) owner[i] = -1;
-  if (threadIdx.x == 0) run_end = num_tokens;
-  __syncthreads();
-  const int slot_base = group * c.group;
-  for (int at = token0;; at += kThreads) {
-    const int i = at + threadIdx.x;
-    if (i < num_tokens) {
-      const int s = slots[i];
-      if (s < slot_base || s - slot_base >= c.group) atomicMin(&run_end, i);
-    }
-    __syncthreads();
-    const int end = run_end;
-    __syncthreads();
-    if (i < end && i < num_tokens) atomicMax(&owner[slots[i] - slot_base], i);
-    if (end < at + kThreads || at + kThreads >= num_tokens) break;
-  }
-  __syncthreads();
+  const int first = blockIdx.x * chunk;
+  auto group_at = [&](int token) {  // -1 where the token is skipped or none
+    if (token < 0 || token >= num_tokens) return -1;
+    const int s = slots[token];
+    return s < 0 || s >= cache_slots ? -1 : c.group_of(s);
+  };
+  const int mine = lane < chunk ? group_at(first + lane) : -1, before = lane < chunk ? group_at(first + lane - 1) : -1;
+  uint64_t begins = __ballot(mine >= 0 && mine != before);
 
   const T* src = (is_v ? value : key) + (int64_t)head * c.head_dim;
   const int64_t src_stride = is_v ? value_stride : key_stride;
-  uint8_t* codes = (is_v ? c.v : c.k) + ((int64_t)slot_base * c.heads + head) * c.head_dim;
   const int64_t row_bytes = (int64_t)c.heads * c.head_dim;
-  float* scale = (is_v ? c.v_scale : c.k_scale) + (int64_t)group * c.heads + head;
-  const int pieces = c.head_dim / 8;  // a thread's step: 8 elements of a row
-  float amax = 0.0f;
-  for (int i = threadIdx.x; i < c.group * pieces; i += kThreads) {
-    const int row = i / pieces, at = (i - row * pieces) * 8, token = owner[row];
-    if (token < 0) continue;
-    float x[8];
-    load_vec<T, 8>(src + token * src_stride + at, x);
+  const int at = (tid & ((1 << lane_bits) - 1)) * 8, row0 = tid >> lane_bits, row_step = kThreads >> lane_bits;
+  const bool in_row = at < c.head_dim;
+  for (; begins; begins &= begins - 1) {
+    const int nth = __ffsll((unsigned long long)begins) - 1;
+    const int token0 = first + nth, group = __shfl(mine, nth);
+    float* scale = (is_v ? c.v_scale : c.k_scale) + (int64_t)group * c.heads + head;
+    const float scale_before = *scale;
+    const int slot_base = group * c.group;
+    for (int i = tid; i < c.group; i += kThreads) owner[i] = -1;
+    for (int from = token0;; from += kThreads) {
+      const int i = from + tid;
+      const int s = i < num_tokens ? slots[i] : -1;
+      const bool in_group = s >= slot_base && s - slot_base < c.group;
+      const uint64_t out = ~__ballot(in_group);
+      if (lane == 0) wave_end[wave] = out ? wave * kWave + __ffsll((unsigned long long)out) - 1 : kThreads;
+      __syncthreads();
+      int end = kThreads;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(x[j]));
-  }
-  amax = wave_max(amax);
-  if (threadIdx.x % kWave == 0) wave_amax[threadIdx.x / kWave] = amax;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / kWave; ++i) amax = fmaxf(amax, wave_amax[i]);
-  float held = 0.0f;
-  if (owner[0] < 0) {
-    const float before = *scale;
-    if (before > 0.0f && before < INFINITY) held = before;
-  }
-  const float fit = fmaxf(scale_for(amax), held);
-  const float inverse = 1.0f / fit;
-  const bool grew = held > 0.0f && fit > held;
-  const float shrink = held / fit;
-  __syncthreads();  // every thread has read the scale
-  if (threadIdx.x == 0) *scale = fit;
-  for (int i = threadIdx.x; i < c.group * pieces; i += kThreads) {
-    const int row = i / pieces, at = (i - row * pieces) * 8, token = owner[row];
-    uint8_t* dst = codes + row * row_bytes + at;
-    u32x2 out;
-    if (token >= 0) {
-      float x[8];
-      load_vec<T, 8>(src + token * src_stride + at, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= inverse;
-      out.x = encode4(x[0], x[1], x[2], x[3]);
-      out.y = encode4(x[4], x[5], x[6], x[7]);
-    } else if (grew) {
-      const u32x2 old = *reinterpret_cast<const u32x2*>(dst);
-      float x[8];
-      decode4(old.x, x);
-      decode4(old.y, x + 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= shrink;
-      out.x = encode4(x[0], x[1], x[2], x[3]);
-      out.y = encode4(x[4], x[5], x[6], x[7]);
-    } else {
-      continue;
+      for (int w = kThreads / kWave - 1; w >= 0; --w)
+        if (wave_end[w] < (w + 1) * kWave) end = wave_end[w];
+      if (tid < end) atomicMax(&owner[s - slot_base], i);
+      __syncthreads();
+      if (end < kThreads) break;
     }
-    *reinterpret_cast<u32x2*>(dst) = out;
+
+    Eight<T> held[kHold];
+    float amax = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kHold; ++p) {
+      const int row = row0 + p * row_step, token = row < c.group && in_row ? owner[row] : -1;
+      if (token < 0) continue;
+      held[p] = *reinterpret_cast<const Eight<T>*>(src + token * src_stride + at);
+    }
+#pragma unroll
+    for (int p = 0; p < kHold; ++p) {
+      const int row = row0 + p * row_step, token = row < c.group && in_row ? owner[row] : -1;
+      if (token < 0) continue;
+      float x[8];
+      expand<T>(held[p], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(x[j]));
+    }
+    for (int row = row0 + kHold * row_step; row < c.group; row += row_step) {
+      const int token = in_row ? owner[row] : -1;
+      if (token < 0) continue;
+      float x[8];
+      expand<T>(*reinterpret_cast<const Eight<T>*>(src + token * src_stride + at), x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(x[j]));
+    }
+    amax = wave_max(amax);
+    if (lane == 0) wave_amax[wave] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) amax = fmaxf(amax, wave_amax[w]);
+    const float kept = owner[0] < 0 && scale_before > 0.0f && scale_before < INFINITY ? scale_before : 0.0f;
+    const float fit = fmaxf(scale_for(amax), kept), inverse = 1.0f / fit, shrink = kept / fit;
+    const bool grew = kept > 0.0f && fit > kept;
+    if (tid == 0) *scale = fit;
+    uint8_t* codes = (is_v ? c.v : c.k) + ((int64_t)slot_base * c.heads + head) * c.head_dim + at;
+    auto write = [&](int row, const Eight<T>* held_row) {
+      const int token = row < c.group && in_row ? owner[row] : -1;
+      u32x2* dst = reinterpret_cast<u32x2*>(codes + row * row_bytes);
+      float x[8];
+      if (token >= 0) {
+        expand<T>(held_row ? *held_row : *reinterpret_cast<const Eight<T>*>(src + token * src_stride + at), x);
+        *dst = encode8(x, inverse);
+      } else if (grew && row < c.group && in_row) {
+        decode4(dst->x, x);
+        decode4(dst->y, x + 4);
+        *dst = encode8(x, shrink);
+      }
+    };
+#pragma unroll
+    for (int p = 0; p < kHold; ++p) write(row0 + p * row_step, &held[p]);
+    for (int row = row0 + kHold * row_step; row < c.group; row += row_step) write(row, nullptr);
+    __syncthreads();  // before the next group's owners
   }
 }
 
 // ---------------------------------------------------------------------------
 // The tokens to keep: for one (sequence, KV head), the last `recent` and the
-// (keep - recent) of the earlier ones with the largest weight. A radix select
-// finds the smallest weight that is kept, 8 bits of its ordered pattern a
-// pass; the kept tokens are then written in order of their position, equal
-// weights by the lowest.
+// (keep - recent) of the earlier ones with the largest weight. The smallest
+// weight that is kept is found two bits at a time of the weights' ordered patterns: the
+// greatest pattern that at least as many reach as are wanted. The kept tokens
+// are then written in order of their position, of equal weights the first.
+// A workgroup takes a row, and a wave a contiguous part of it. kHeld: up to 32
+// weights a lane stay in registers throughout, so that two bits cost three
+// comparisons and scalar bit counts for each 64 weights and one barrier (bit by
+// bit, the barriers made it 18.6 and 33.1 us for rows of 8,192 and 32,767); rows
+// of more than 32,768 are read again for each two. The search ends early where exactly as
+// many are reached as wanted, and leaves out bits that all patterns share. (A
+// radix select by histograms in LDS took 21 and 46 us for rows of 8,192 and
+// 32,767: weights crowd in few bins, and additions to one address take turns.)
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
+constexpr int kSelectHeld = 32;
 
 // Orders as the weights do: -0 as +0, NaN below everything.
 __device__ __forceinline__ uint32_t rank_of(float w) {
@@ -265,122 +307,181 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float weight_of(uint32_t rank) {
+  return rank == 0 ? NAN : __uint_as_float(rank & 0x80000000u ? rank ^ 0x80000000u : ~rank);
+}
+
+template <bool kHeld>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(const float* __restrict__ weights, int32_t heads,
                                                                 int32_t width, const int32_t* __restrict__ lens,
                                                                 int32_t keep, int32_t recent,
                                                                 int32_t* __restrict__ indices,
                                                                 int32_t* __restrict__ counts,
                                                                 float* __restrict__ kept) {
-  __shared__ uint32_t bins[256];
-  __shared__ uint32_t chosen, above;
-  __shared__ uint32_t wave_over[kSelectWaves], wave_tied[kSelectWaves];
+  __shared__ uint32_t reached[16][3], varying[2];
+  __shared__ uint32_t wave_a[kSelectWaves], wave_b[kSelectWaves];
   const int64_t row = blockIdx.x;
-  const int seq = (int)(row / heads), tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const int seq = (int)(row / heads), tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const float* w = weights + row * width;
   int32_t* out = indices + row * keep;
   float* out_w = kept + row * keep;
   int n = lens[seq];
   n = n < 0 ? 0 : n > width ? width : n;
   const int count = n < keep ? n : keep;
+  const int last = recent < count ? recent : count;  // kept at the end whatever they weigh
+  const int pool = n - last, want = count - last;    // of the first `pool`, `want` are kept
   if (tid == 0 && row % heads == 0) counts[seq] = count;
   for (int i = count + tid; i < keep; i += kSelectThreads) {
     out[i] = -1;
     out_w[i] = 0.0f;
   }
-  const int last = recent < count ? recent : count;  // kept at the end whatever they weigh
-  const int pool = n - last, want = count - last;    // of the first `pool`, `want` are kept
-  uint32_t prefix = 0, need = (uint32_t)want;
-  if (want > 0 && want < pool) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) bins[tid] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0 : ~0u << (shift + 8);
-      for (int i = tid; i < pool; i += kSelectThreads) {
-        const uint32_t r = rank_of(w[i]);
-        if ((r & mask) == prefix) atomicAdd(&bins[(r >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (wave == 0) {
-        // Lane l sums bins 255 - 4 l .. 252 - 4 l; a scan over the lanes finds the bin that holds the need-th largest.
-        uint32_t b[4], total = 0;
-        for (int j = 0; j < 4; ++j) total += b[j] = bins[255 - (lane * 4 + j)];
-        uint32_t before = total;
-        for (int d = 1; d < kWave; d <<= 1) {
-          const uint32_t other = __shfl_up(before, d);
-          if (lane >= d) before += other;
-        }
-        before -= total;
-        if (before < need && need <= before + total) {
-          for (int j = 0; j < 4; ++j) {
-            if (before < need && need <= before + b[j]) {
-              chosen = (uint32_t)(255 - (lane * 4 + j));
-              above = before;
-            }
-            before += b[j];
-          }
-        }
-      }
-      __syncthreads();
-      prefix |= chosen << shift;
-      need -= above;
-    }
-  }
-  // Over the threshold, or tied with it and among the first `need`.
-  const bool all = want >= pool;
-  uint32_t placed = 0, tied = 0;
-  if (want > 0) {
-    for (int base = 0; base < pool; base += kSelectThreads) {
-      const int i = base + tid;
-      const float x = i < pool ? w[i] : 0.0f;
-      const uint32_t r = rank_of(x);
-      const bool over = i < pool && (all || r > prefix), tie = i < pool && !all && r == prefix;
-      const uint64_t over_mask = __ballot(over), tie_mask = __ballot(tie);
-      if (lane == 0) {
-        wave_over[wave] = __popcll(over_mask);
-        wave_tied[wave] = __popcll(tie_mask);
-      }
-      __syncthreads();
-      const uint64_t below = (uint64_t{1} << lane) - 1;
-      uint32_t overs = __popcll(over_mask & below), ties = __popcll(tie_mask & below), all_over = 0, all_tied = 0;
-      for (int j = 0; j < kSelectWaves; ++j) {
-        const uint32_t o = wave_over[j], t = wave_tied[j];
-        if (j < wave) {
-          overs += o;
-          ties += t;
-        }
-        all_over += o;
-        all_tied += t;
-      }
-      const uint32_t tie_rank = tied + ties;
-      if (over || (tie && tie_rank < need)) {
-        const uint32_t at = placed + overs + (tie_rank < need ? tie_rank : need) - (tied < need ? tied : need);
-        out[at] = i;
-        out_w[at] = x;
-      }
-      const uint32_t taken_before = tied < need ? tied : need;
-      tied += all_tied;
-      placed += all_over + (tied < need ? tied : need) - taken_before;
-      __syncthreads();
-    }
-  }
   for (int i = tid; i < last; i += kSelectThreads) {
     out[want + i] = pool + i;
     out_w[want + i] = w[pool + i];
   }
+  if (want == pool) {
+    for (int i = tid; i < pool; i += kSelectThreads) {
+      out[i] = i;
+      out_w[i] = w[i];
+    }
+    return;
+  }
+  if (want == 0) return;
+
+  // The wave's part: [first, first + 64 per), as far as it lies within the pool. Past that, patterns are 0: no candidate
+  // is reached by them, and of equal ones they come last (those of j >= per are left out).
+  const int per = (pool + kSelectThreads - 1) / kSelectThreads, first = wave * per * kWave;
+  auto read = [&](int j) {
+    const int i = first + j * kWave + lane;
+    return i < pool ? rank_of(w[i]) : 0u;
+  };
+  uint32_t held[kHeld ? kSelectHeld : 1];
+  uint32_t set = 0, clear = 0;  // bits that are set, and clear, in some pattern
+  if constexpr (kHeld) {
+    // Whole loads first, from places within the row: behind a condition each would be waited for in turn.
+#pragma unroll
+    for (int j = 0; j < kSelectHeld; ++j) {
+      const int i = first + j * kWave + lane;
+      held[j] = __float_as_uint(w[i < pool ? i : pool - 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < kSelectHeld; ++j) {
+      const bool in = j < per && first + j * kWave + lane < pool;
+      held[j] = in ? rank_of(__uint_as_float(held[j])) : 0u;
+      set |= held[j];
+      clear |= in ? ~held[j] : 0u;
+    }
+  } else {
+    for (int j = 0; j < per; ++j) {
+      const uint32_t r = read(j);
+      set |= r;
+      clear |= first + j * kWave + lane < pool ? ~r : 0u;
+    }
+  }
+  // body(j, pattern) for each j < per, and perhaps some more whose patterns are 0.
+  auto each = [&](auto body) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < kSelectHeld; j += 8) {
+        if (j >= per) break;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) body(j + k, held[j + k]);
+      }
+    } else {
+      for (int j = 0; j < per; ++j) body(j, read(j));
+    }
+  };
+  if (tid < 48) reached[tid / 3][tid % 3] = 0;
+  if (tid < 2) varying[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    set |= __shfl_xor(set, d);
+    clear |= __shfl_xor(clear, d);
+  }
+  if (lane == 0) {
+    atomicOr(&varying[0], set);
+    atomicOr(&varying[1], clear);
+  }
+  __syncthreads();
+  uint32_t always = varying[0] & ~varying[1], open = varying[0] & varying[1];
+  uint32_t prefix = 0, found = (uint32_t)pool;  // as many reach `prefix`
+  for (int low = 30; low >= 0 && found != (uint32_t)want; low -= 2) {
+    if (!(open >> low & 3)) {
+      prefix |= always & 3u << low;
+      continue;
+    }
+    uint32_t mine[3] = {0, 0, 0};
+    each([&](int, uint32_t r) {
+#pragma unroll
+      for (uint32_t i = 0; i < 3; ++i) mine[i] += (uint32_t)__popcll(__ballot(r >= (prefix | (i + 1) << low)));
+    });
+    if (lane < 3) atomicAdd(&reached[low / 2][lane], lane == 0 ? mine[0] : lane == 1 ? mine[1] : mine[2]);
+    __syncthreads();
+    uint32_t digit = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i) {
+      const uint32_t all = reached[low / 2][i];
+      if (all >= (uint32_t)want) {
+        digit = i + 1;
+        found = all;
+      }
+    }
+    prefix |= digit << low;
+  }
+  // Kept: all that reach it, where those are as many as wanted; else what is above it, and of those equal to it, the
+  // smallest weight that is kept, the first ones.
+  const bool exact = found == (uint32_t)want;
+  if (exact) --prefix;  // `above it` then, and none equal; it is not 0, which all reach
+  uint32_t my_overs = 0, my_ties = 0;
+  each([&](int j, uint32_t r) {
+    my_overs += (uint32_t)__popcll(__ballot(r > prefix));
+    my_ties += (uint32_t)__popcll(__ballot(j < per && r == prefix));
+  });
+  if (lane == 0) {
+    wave_a[wave] = my_overs;
+    wave_b[wave] = my_ties;
+  }
+  __syncthreads();
+  uint32_t over_at = 0, tie_at = 0, need = (uint32_t)want;
+  for (int i = 0; i < kSelectWaves; ++i) {
+    if (i < wave) {
+      over_at += wave_a[i];
+      tie_at += wave_b[i];
+    }
+    need -= wave_a[i];
+  }
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  each([&](int j, uint32_t r) {
+    const bool over = r > prefix, tie = j < per && r == prefix;
+    const uint64_t over_mask = __ballot(over), tie_mask = __ballot(tie);
+    const uint32_t tie_rank = tie_at + (uint32_t)__popcll(tie_mask & below);
+    if (over || (tie && tie_rank < need)) {
+      const uint32_t at = over_at + (uint32_t)__popcll(over_mask & below) + (tie_rank < need ? tie_rank : need);
+      out[at] = first + j * kWave + lane;
+      out_w[at] = weight_of(r);  // loaded again, it would be waited for in each turn: 17.1 and 35.1 us
+    }
+    over_at += (uint32_t)__popcll(over_mask);
+    tie_at += (uint32_t)__popcll(tie_mask);
+  });
 }
 
 // ---------------------------------------------------------------------------
 // Compaction: a workgroup gathers the rows of one group of the new blocks, for
-// one head of K or V, and encodes them under a scale of their own.
+// one head of K or V, and encodes them under a scale of their own. As in the
+// cache write, a thread keeps the pieces that it read, of 16 codes here.
 
 __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatch from,
                                                            const int32_t* __restrict__ indices,
                                                            const int32_t* __restrict__ counts, int32_t keep,
                                                            const int32_t* __restrict__ to_tables, int64_t to_stride,
-                                                           int32_t to_width) {
+                                                           int32_t to_width, int32_t lane_bits) {
+  constexpr int kHold = 2;
   __shared__ float wave_amax[kThreads / kWave];
   __shared__ int64_t source[kMaxGroup];  // slot of each row, or -1
-  const int head = blockIdx.y % c.heads, seq = blockIdx.z;
+  __shared__ float source_scale[kMaxGroup];
+  const int tid = threadIdx.x, head = blockIdx.y % c.heads, seq = blockIdx.z;
   const bool is_v = blockIdx.y >= c.heads;
   int count = counts[seq];
   count = count < 0 ? 0 : count > keep ? keep : count;
@@ -391,60 +492,73 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   if (to_block >= to_width) return;
   const int target = to_tables[seq * to_stride + to_block];
   if (target < 0 || target >= c.num_blocks) return;
+  uint8_t* codes = is_v ? c.v : c.k;
+  float* scales = is_v ? c.v_scale : c.k_scale;
   const int64_t to_slot = (int64_t)target * c.block_size + (first - to_block * c.block_size);
   const int32_t* mine = indices + ((int64_t)seq * c.heads + head) * keep + first;
   const int context = context_of(from, seq, c.block_size);
-  for (int i = threadIdx.x; i < rows; i += kThreads) {
+  for (int i = tid; i < rows; i += kThreads) {
     const int t = mine[i];
     int64_t slot = -1;
+    float scale = 0.0f;
     if (t >= 0 && t < context) {
-      const int b = c.block_of(t);
+      const int b = c.block_of(t), in = t - b * c.block_size;
       const int id = from.tables[seq * from.table_stride + b];
-      if (id >= 0 && id < c.num_blocks) slot = (int64_t)id * c.block_size + (t - b * c.block_size);
+      if (id >= 0 && id < c.num_blocks) {
+        slot = (int64_t)id * c.block_size + in;
+        scale = scales[((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head];
+      }
     }
     source[i] = slot;
+    source_scale[i] = scale;
   }
   __syncthreads();
-  uint8_t* codes = is_v ? c.v : c.k;
-  float* scales = is_v ? c.v_scale : c.k_scale;
-  const int pieces = c.head_dim / 8;
+  const int at = (tid & ((1 << lane_bits) - 1)) * 16, row0 = tid >> lane_bits, row_step = kThreads >> lane_bits;
+  const bool in_row = at < c.head_dim;
+  auto read = [&](int row) {
+    u32x4 w = {0, 0, 0, 0};
+    if (row < rows && in_row && source[row] >= 0)
+      w = *reinterpret_cast<const u32x4*>(codes + (source[row] * c.heads + head) * c.head_dim + at);
+    return w;
+  };
+  auto value = [&](const u32x4& w, float scale, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) decode4(w[i], x + 4 * i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= scale;
+  };
+  auto amax_of = [&](const u32x4& w, int row) {
+    float x[16], most = 0.0f;
+    value(w, row < rows ? source_scale[row] : 0.0f, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, finite_abs(x[i]));
+    return most;
+  };
+  u32x4 held[kHold];
   float amax = 0.0f;
-  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
-    const int row = i / pieces, at = (i - row * pieces) * 8;
-    const int64_t slot = source[row];
-    if (slot < 0) continue;
-    const float s = scales[(slot / c.group) * c.heads + head];
-    const u32x2 w = *reinterpret_cast<const u32x2*>(codes + (slot * c.heads + head) * c.head_dim + at);
-    float x[8];
-    decode4(w.x, x);
-    decode4(w.y, x + 4);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(x[j] * s));
-  }
+  for (int p = 0; p < kHold; ++p) held[p] = read(row0 + p * row_step);
+#pragma unroll
+  for (int p = 0; p < kHold; ++p) amax = fmaxf(amax, amax_of(held[p], row0 + p * row_step));
+  for (int row = row0 + kHold * row_step; row < rows; row += row_step) amax = fmaxf(amax, amax_of(read(row), row));
   amax = wave_max(amax);
-  if (threadIdx.x % kWave == 0) wave_amax[threadIdx.x / kWave] = amax;
+  if (tid % kWave == 0) wave_amax[tid / kWave] = amax;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / kWave; ++i) amax = fmaxf(amax, wave_amax[i]);
+  for (int w = 0; w < kThreads / kWave; ++w) amax = fmaxf(amax, wave_amax[w]);
   const float fit = scale_for(amax), inverse = 1.0f / fit;
-  if (threadIdx.x == 0) scales[(to_slot / c.group) * c.heads + head] = fit;
-  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
-    const int row = i / pieces, at = (i - row * pieces) * 8;
-    const int64_t slot = source[row];
-    u32x2 out = {0, 0};
-    if (slot >= 0) {
-      const float s = scales[(slot / c.group) * c.heads + head];
-      const u32x2 w = *reinterpret_cast<const u32x2*>(codes + (slot * c.heads + head) * c.head_dim + at);
-      float x[8];
-      decode4(w.x, x);
-      decode4(w.y, x + 4);
+  if (tid == 0)
+    scales[((int64_t)target * (c.block_size / c.group) + c.group_of(first - to_block * c.block_size)) * c.heads + head] = fit;
+  auto write = [&](const u32x4& w, int row) {
+    if (row >= rows || !in_row) return;
+    float x[16];
+    value(w, source_scale[row], x);
+    const u32x2 lo = encode8(x, inverse), hi = encode8(x + 8, inverse);
+    *reinterpret_cast<u32x4*>(codes + ((to_slot + row) * c.heads + head) * c.head_dim + at) = u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * s * inverse;
-      out.x = encode4(x[0], x[1], x[2], x[3]);
-      out.y = encode4(x[4], x[5], x[6], x[7]);
-    }
-    *reinterpret_cast<u32x2*>(codes + ((to_slot + row) * c.heads + head) * c.head_dim + at) = out;
-  }
+  for (int p = 0; p < kHold; ++p) write(held[p], row0 + p * row_step);
+  for (int row = row0 + kHold * row_step; row < rows; row += row_step) write(read(row), row);
 }
 
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
@@ -465,11 +579,17 @@ hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Up to so many tokens each is looked at by workgroups of its own, as a decode step's begin a group each.
+constexpr int kStoreSingle = 1024;
+
 template <typename T>
 hipError_t store_of(const Fp8Cache& c, const void* key, int64_t key_stride, const void* value, int64_t value_stride,
                     const int32_t* slots, int32_t num_tokens, hipStream_t stream) {
-  store_fp8_kernel<T><<<dim3((unsigned)num_tokens, (unsigned)(2 * c.heads)), dim3(kThreads), 0, stream>>>(
-      c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens);
+  int lane_bits = 1;
+  while ((8 << lane_bits) < c.head_dim) ++lane_bits;
+  const int chunk = num_tokens <= kStoreSingle ? 1 : 16;
+  store_fp8_kernel<T><<<dim3((unsigned)((num_tokens + chunk - 1) / chunk), (unsigned)(2 * c.heads)), dim3(kThreads), 0, stream>>>(
+      c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens, chunk, lane_bits);
   return hipGetLastError();
 }
 
@@ -493,8 +613,11 @@ hipError_t launch_store_fp8(const Fp8Cache& c, const void* key, int64_t key_stri
 hipError_t launch_select(const float* weights, int32_t rows, int32_t heads, int32_t width, const int32_t* context_lens,
                          int32_t keep, int32_t recent, int32_t* indices, int32_t* counts, float* kept,
                          hipStream_t stream) {
-  select_kernel<<<dim3((unsigned)rows), dim3(kSelectThreads), 0, stream>>>(weights, heads, width, context_lens, keep,
-                                                                         recent, indices, counts, kept);
+  const dim3 grid((unsigned)rows), block(kSelectThreads);
+  if (width <= kSelectThreads * kSelectHeld)
+    select_kernel<true><<<grid, block, 0, stream>>>(weights, heads, width, context_lens, keep, recent, indices, counts, kept);
+  else
+    select_kernel<false><<<grid, block, 0, stream>>>(weights, heads, width, context_lens, keep, recent, indices, counts, kept);
   return hipGetLastError();
 }
 
@@ -502,7 +625,10 @@ hipError_t launch_compact(const Fp8Cache& c, const PagedBatch& from, const int32
                           int32_t keep, const int32_t* to_tables, int64_t to_stride, int32_t to_width,
                           hipStream_t stream) {
   const dim3 grid((unsigned)((keep + c.group - 1) / c.group), (unsigned)(2 * c.heads), (unsigned)from.num_seqs);
-  compact_kernel<<<grid, dim3(kThreads), 0, stream>>>(c, from, indices, counts, keep, to_tables, to_stride, to_width);
+  int lane_bits = 0;
+  while ((16 << lane_bits) < c.head_dim) ++lane_bits;
+  compact_kernel<<<grid, dim3(kThreads), 0, stream>>>(c, from, indices, counts, keep, to_tables, to_stride, to_width,
+                                                      lane_bits);
   return hipGetLastError();
 }
 

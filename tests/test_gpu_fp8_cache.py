@@ -524,6 +524,27 @@ def test_selected_tokens(gpu, kind, width, keep, recent):
                            y.nan_to_num(-7.0) if y.is_floating_point() else y)
 
 
+@pytest.mark.parametrize("pool", [3, 70, 5000])
+def test_weights_that_are_no_numbers_come_last(gpu, pool):
+    weights = torch.full((1, 1, pool), math.nan)
+    weights[0, 0, pool // 2] = 5.0
+    for keep in (1, 2, pool - 1):
+        got = ops.select_tokens(weights.to(gpu), int32([pool], gpu), keep)
+        want = ref.select(weights, [pool], keep, 0)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[2].cpu().nan_to_num(-7.0), want[2].nan_to_num(-7.0))
+
+
+@pytest.mark.parametrize("kind", ["random", "few", "equal"])
+@pytest.mark.parametrize("width", [32768, 32769])
+def test_selected_tokens_about_the_longest_held_row(gpu, width, kind):
+    weights = torch.rand((1, 1, width), generator=torch.Generator().manual_seed(2))
+    weights = (weights * 3).floor() if kind == "few" else weights * 0 if kind == "equal" else weights
+    for keep, recent in ((width - 1, 0), (17, 3), (20000, 1)):
+        got = ops.select_tokens(weights.to(gpu), int32([width], gpu), keep, recent)
+        for x, y in zip(got, ref.select(weights, [width], keep, recent)):
+            assert torch.equal(x.cpu(), y)
+
+
 def test_selected_tokens_of_a_long_context(gpu):
     weights = (torch.rand((1, 2, 70001), generator=torch.Generator().manual_seed(2)) * 500).round() / 500
     got = ops.select_tokens(weights.to(gpu), int32([69999], gpu), 9001, 1000)
