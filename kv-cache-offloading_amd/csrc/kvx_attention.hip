@@ -921,29 +921,70 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttentionArgs a) {
 
 // ---------------------------------------------------------------------------
 // The weight of each cached token: out = weights + the sum over the query rows
-// of exp(score - lse). A wave holds 32 keys' K and passes over all query rows.
+// that see it of exp(score - lse). A key belongs to one wave, which passes over
+// all query rows in order: no atomics, one order of the sums.
 
-// 16 keys that lie in one block and under one scale: where their rows begin,
-// or nothing where the keys are past the context or their block is no block.
-struct Tile {
-  int64_t row;   // slot * heads + head of the first key
-  int64_t scale; // element of the scales
-  bool there;
+// The query row r of a (sequence, KV head): its address, its last key, and its lse over log(2); infinity, which makes
+// every weight 0, where there is no such row or it sees nothing.
+template <typename T>
+struct WeightRow {
+  const T* query;
+  float lse;
+  int last;
 };
-__device__ __forceinline__ Tile tile_at(const Fp8Cache& c, const int32_t* table, int key, int context, int head) {
-  Tile t = {0, 0, false};
-  if (key >= context) return t;
-  const int nth = c.block_of(key), in = key - nth * c.block_size;
-  const int id = __builtin_amdgcn_readfirstlane(table[nth]);
-  if (id < 0 || id >= c.num_blocks) return t;
-  t.row = ((int64_t)id * c.block_size + in) * c.heads + head;
-  t.scale = ((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head;
-  t.there = true;
-  return t;
+template <typename T>
+__device__ __forceinline__ WeightRow<T> weight_row(const WeightsArgs& a, const QueryRows& rows, int context, int head,
+                                                   int r) {
+  const bool real = r < rows.count * a.per_kv;
+  const int nth = real ? (int)a.per_kv_of(r) : 0, q_head = head * a.per_kv + (real ? r - nth * a.per_kv : 0);
+  WeightRow<T> row;
+  row.query = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride + (int64_t)q_head * a.cache.head_dim;
+  row.last = real ? context - rows.count + nth : -1;
+  const float lse = real ? a.lse[(int64_t)(rows.first + nth) * a.q_heads + q_head] : -INFINITY;
+  row.lse = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+  return row;
 }
 
-template <int kType, int kHd>
-__global__ __launch_bounds__(kThreads) void weights_kernel(WeightsArgs a) {
+// 16 adjacent keys' lookup, a lane for each.
+struct KeyTile {
+  int64_t row;  // slot * heads + head of the first key, or -1
+  float scale;
+};
+__device__ __forceinline__ KeyTile key_tile(const WeightsArgs& a, const int32_t* table, int context, int head, int key) {
+  const Fp8Cache& cache = a.cache;
+  KeyTile t = {-1, 0.0f};
+  if (key < context) {
+    const int block = cache.block_of(key), in = key - block * cache.block_size;
+    const int id = table[block];
+    if (id >= 0 && id < cache.num_blocks) {
+      t.row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
+      t.scale = cache.k_scale[((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head] *
+                a.scale;
+    }
+  }
+  return t;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// The sum over the 16 lanes of a row, in all of them.
+__device__ __forceinline__ float sum16(float x) {
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));  // row_ror:8
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xF, 0xF, false));
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xF, 0xF, false));
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xF, 0xF, false));
+}
+
+// Few query rows: bound by the bytes of K. A wave asks for kTiles * 16 keys at
+// once; its query rows come straight from memory, 16 at a time.
+template <int kType, int kHd, int kTiles>
+__global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
   using Q = Query<kType>;
   using T = typename Q::T;
   using Vec = typename Q::Vec;
@@ -952,78 +993,227 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsArgs a) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int pairs = a.batch.num_seqs * cache.heads;
-  const int pair = blockIdx.x % pairs;
-  const int seq = pair / cache.heads, head = pair % cache.heads;
-  const QueryRows rows = query_rows(a.batch, seq);
-  const int context = context_of(a.batch, seq, cache.block_size);
-  const int num_rows = rows.count * a.per_kv;
-  const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
-  const int64_t base = (int64_t)pair * a.width;
-  const int key0 = ((blockIdx.x / pairs) * kWaves + wave) * kStep;
+  const int pair = blockIdx.x % pairs, seq = pair / cache.heads, head = pair % cache.heads;
+  const int key0 = ((blockIdx.x / pairs) * kWaves + wave) * kTiles * 16;
   if (key0 >= a.width) return;
-  float total[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) total[j] = 0.0f;
-  if (key0 < context) {
-    const Tile tiles[2] = {tile_at(cache, table, key0, context, head), tile_at(cache, table, key0 + 16, context, head)};
-    Vec k[2][2 * kChunks];
-    float ks[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t* p = cache.k + (tiles[t].row + (int64_t)c * cache.heads) * cache.head_dim;
-      ks[t] = tiles[t].there ? cache.k_scale[tiles[t].scale] * a.scale : 0.0f;
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int at = i * 64 + g * 16;
-        u32x4 w = {0, 0, 0, 0};
-        if (tiles[t].there && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(p + at);
-        k[t][2 * i] = decode8<Q>(w.x, w.y);
-        k[t][2 * i + 1] = decode8<Q>(w.z, w.w);
-      }
+  const int context = context_of(a.batch, seq, cache.block_size);
+  const int64_t base = (int64_t)pair * a.width;
+  if (key0 >= context) {  // nothing is added
+    if (a.weights != a.out) {
+      for (int key = key0 + lane; key < key0 + kTiles * 16 && key < a.width; key += kWave)
+        a.out[base + key] = a.weights ? a.weights[base + key] : 0.0f;
     }
-    // Rows before this one see none of the keys.
-    const int first_query = key0 - (context - rows.count);
-    const int first_row = first_query > 0 ? first_query * a.per_kv / 16 * 16 : 0;
-    for (int row0 = first_row; row0 < num_rows; row0 += 16) {
-      const int r = row0 + c;
-      const bool real = r < num_rows;
-      const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
-      const int last = real ? context - rows.count + nth : -1;
-      const int q_head = head * a.per_kv + sub;
-      const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride + (int64_t)q_head * cache.head_dim;
-      const float lse = real ? a.lse[(int64_t)(rows.first + nth) * a.q_heads + q_head] * 1.4426950408889634f : 0.0f;
-      f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int at = i * 64 + g * 16;
-        u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-        if (real && at < cache.head_dim) {
-          lo = *reinterpret_cast<const u32x4*>(src + at);
-          hi = *reinterpret_cast<const u32x4*>(src + at + 8);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          s[t] = Q::mfma(k[t][2 * i], __builtin_bit_cast(Vec, lo), s[t]);
-          s[t] = Q::mfma(k[t][2 * i + 1], __builtin_bit_cast(Vec, hi), s[t]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool see = key0 + (j / 4) * 16 + 4 * g + j % 4 <= last && tiles[j / 4].there && lse != -INFINITY;
-        total[j] += see ? exp2f(s[j / 4][j % 4] * ks[j / 4] - lse) : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) total[j] += __shfl_xor(total[j], d);
+    return;
   }
-  if (c == 0) {
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int num_rows = rows.count * a.per_kv;
+  WeightRow<T> row = weight_row<T>(a, rows, context, head, c);
+  const KeyTile mine = key_tile(a, a.batch.tables + seq * a.batch.table_stride, lane < kTiles ? context : 0, head,
+                                key0 + lane * 16);
+  const int32_t k_lane = c * cache.heads * cache.head_dim + g * 16;
+  u32x4 k[kTiles][kChunks];
+  float scale[kTiles];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = key0 + (j / 4) * 16 + 4 * g + j % 4;
-      if (key < a.width) a.out[base + key] = (a.weights ? a.weights[base + key] : 0.0f) + total[j];
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t at = lane_value(mine.row, t);
+    scale[t] = lane_value(mine.scale, t);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      k[t][i] = u32x4{0, 0, 0, 0};
+      if (at >= 0 && i * 64 + g * 16 < cache.head_dim)
+        k[t][i] = *reinterpret_cast<const u32x4*>(cache.k + at * cache.head_dim + (k_lane + i * 64));
     }
+  }
+  // Lane (c, g) writes keys 4 g + i of tile c.
+  float before[4] = {0, 0, 0, 0}, total[kTiles][4];
+  const int my_key = key0 + c * 16 + 4 * g;
+  if (a.weights && c < kTiles) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) before[i] = a.weights[base + (my_key + i < a.width ? my_key + i : 0)];
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total[t][i] = 0.0f;
+  for (int row0 = 0; row0 < num_rows; row0 += 16) {
+    if (row0 > 0) row = weight_row<T>(a, rows, context, head, row0 + c);
+    Vec q[2 * kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int at = i * 64 + g * 16;
+      u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+      if (at < cache.head_dim) {
+        lo = *reinterpret_cast<const u32x4*>(row.query + at);
+        hi = *reinterpret_cast<const u32x4*>(row.query + at + 8);
+      }
+      q[2 * i] = __builtin_bit_cast(Vec, lo);
+      q[2 * i + 1] = __builtin_bit_cast(Vec, hi);
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        s = Q::mfma(decode8<Q>(k[t][i].x, k[t][i].y), q[2 * i], s);
+        s = Q::mfma(decode8<Q>(k[t][i].z, k[t][i].w), q[2 * i + 1], s);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[i] * scale[t] - row.lse);
+        total[t][i] += key0 + t * 16 + 4 * g + i <= row.last ? p : 0.0f;
+      }
+    }
+  }
+  float added[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const bool there = lane_value(mine.row, t) >= 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float sum = sum16(total[t][i]);
+      added[i] = there && c == t ? sum : added[i];
+    }
+  }
+  if (c < kTiles) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (my_key + i < a.width) a.out[base + my_key + i] = before[i] + added[i];
+  }
+}
+
+// Many query rows: bound by the exponentials and the matrix cores. A wave keeps
+// 32 keys' K as operands; the workgroup's waves share the query rows, 64 at a
+// time, through LDS, and a wave computes the scores of the next 32 of them under
+// the exponentials of these.
+template <int kType, int kHd>
+__global__ __launch_bounds__(kThreads) void weights_many_kernel(WeightsArgs a) {
+  using Q = Query<kType>;
+  using T = typename Q::T;
+  using Vec = typename Q::Vec;
+  constexpr int kDots = kHd / 16;
+  constexpr int kRowsHeld = 64;
+  constexpr int kPitch = kHd * 2 + 16;
+  constexpr int kLoads = kRowsHeld * kHd / 8 / kThreads;  // 16-byte pieces of the rows a thread
+  __shared__ alignas(16) uint8_t q_lds[2][kRowsHeld * kPitch];
+  __shared__ float lse_lds[2][kRowsHeld];
+  __shared__ int last_lds[2][kRowsHeld];
+  const Fp8Cache& cache = a.cache;
+  const int tid = threadIdx.x, lane = tid % kWave, n32 = lane % 32, h = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int pairs = a.batch.num_seqs * cache.heads;
+  const int pair = blockIdx.x % pairs, seq = pair / cache.heads, head = pair % cache.heads;
+  const int group0 = (blockIdx.x / pairs) * kWaves * 32, key0 = group0 + wave * 32;
+  const int context = context_of(a.batch, seq, cache.block_size);
+  const int64_t base = (int64_t)pair * a.width;
+  const QueryRows rows = query_rows(a.batch, seq);
+  const int num_rows = group0 < context ? rows.count * a.per_kv : 0;
+
+  const KeyTile mine = key_tile(a, a.batch.tables + seq * a.batch.table_stride, lane < 2 ? context : 0, head,
+                                key0 + lane * 16);
+  const bool there[2] = {lane_value(mine.row, 0) >= 0, lane_value(mine.row, 1) >= 0};
+  const float scale[2] = {lane_value(mine.scale, 0), lane_value(mine.scale, 1)};
+  // K: lane (n, h) holds columns 16 d + 8 h .. of key n.
+  Vec k[kDots];
+  {
+    const int64_t row = n32 < 16 ? lane_value(mine.row, 0) : lane_value(mine.row, 1);
+    const uint8_t* src = cache.k + (row + (int64_t)(n32 % 16) * cache.heads) * cache.head_dim + h * 8;
+    u32x2 raw[kDots];
+#pragma unroll
+    for (int d = 0; d < kDots; ++d) {
+      raw[d] = u32x2{0, 0};
+      if (row >= 0 && d * 16 < cache.head_dim) raw[d] = *reinterpret_cast<const u32x2*>(src + d * 16);
+    }
+#pragma unroll
+    for (int d = 0; d < kDots; ++d) k[d] = decode8<Q>(raw[d].x, raw[d].y);
+  }
+  float total[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) total[i] = 0.0f;
+
+  // Rows before the first that sees a key of the workgroup are left out.
+  const int first_query = num_rows > 0 ? group0 - (context - rows.count) : 0;
+  const int first_row = first_query > 0 ? first_query * a.per_kv / kRowsHeld * kRowsHeld : 0;
+  u32x4 piece[kLoads];
+  float lse = 0.0f;
+  int last = -1;
+  auto load = [&](int row0) {
+    constexpr int kPieces = kHd / 8;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = row0 + (i * kThreads + tid) / kPieces, at = (i * kThreads + tid) % kPieces * 8;
+      const bool real = r < num_rows && at < cache.head_dim;
+      const int nth = real ? (int)a.per_kv_of(r) : 0, sub = real ? r - nth * a.per_kv : 0;
+      piece[i] = u32x4{0, 0, 0, 0};
+      if (real)
+        piece[i] = *reinterpret_cast<const u32x4*>((const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride +
+                                                   (int64_t)(head * a.per_kv + sub) * cache.head_dim + at);
+    }
+    if (tid < kRowsHeld) {
+      const WeightRow<T> row = weight_row<T>(a, rows, context, head, row0 + tid < num_rows ? row0 + tid : INT32_MAX);
+      lse = row.lse;
+      last = row.last;
+    }
+  };
+  auto put = [&](int buffer) {
+    constexpr int kPieces = kHd / 8;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (i * kThreads + tid) / kPieces, at = (i * kThreads + tid) % kPieces * 16;
+      *reinterpret_cast<u32x4*>(q_lds[buffer] + r * kPitch + at) = piece[i];
+    }
+    if (tid < kRowsHeld) {
+      lse_lds[buffer][tid] = lse;
+      last_lds[buffer][tid] = last;
+    }
+  };
+  auto scores = [&](int buffer, int half) {
+    const uint8_t* from = q_lds[buffer] + (half * 32 + n32) * kPitch + h * 16;
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDots; ++d) s = mfma32<kType>(k[d], *reinterpret_cast<const Vec*>(from + d * 32), s);
+    return s;
+  };
+  auto add = [&](float row_lse, int row_last, const f32x16& s) {
+    if (__any(key0 + 31 > row_last)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale[i / 8], -row_lse));
+        total[i] += key0 + 8 * (i / 4) + 4 * h + i % 4 <= row_last ? p : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) total[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale[i / 8], -row_lse));
+    }
+  };
+  if (first_row < num_rows) {
+    load(first_row);
+    put(0);
+    __syncthreads();
+    int buffer = 0;
+    f32x16 s = scores(0, 0);
+    for (int row0 = first_row; row0 < num_rows; row0 += kRowsHeld, buffer ^= 1) {
+      const bool more = row0 + kRowsHeld < num_rows;
+      if (more) load(row0 + kRowsHeld);
+      const f32x16 second = scores(buffer, 1);
+      add(lse_lds[buffer][n32], last_lds[buffer][n32], s);
+      if (more) put(buffer ^ 1);
+      // Read before the barrier, behind which the next turn's rows but one may replace them.
+      const float second_lse = lse_lds[buffer][32 + n32];
+      const int second_last = last_lds[buffer][32 + n32];
+      __syncthreads();
+      if (more) s = scores(buffer ^ 1, 0);
+      add(second_lse, second_last, second);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float sum = sum16(total[i]);
+    sum += __shfl_xor(sum, 16);
+    const int key = key0 + 8 * (i / 4) + 4 * h + i % 4;
+    if (n32 == i && key < a.width)
+      a.out[base + key] = (a.weights ? a.weights[base + key] : 0.0f) + (there[i / 8] && key < context ? sum : 0.0f);
   }
 }
 
@@ -1077,16 +1267,29 @@ hipError_t attention_sized(const AttentionArgs& a, hipStream_t stream) {
   }
 }
 
-template <int kType>
-hipError_t weights_sized(const WeightsArgs& a, hipStream_t stream) {
-  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * ((a.width + kWaves * kStep - 1) / (kWaves * kStep));
-  const dim3 g((unsigned)grid), b(kThreads);
-  switch (padded_head(a.cache.head_dim)) {
-    case 64: weights_kernel<kType, 64><<<g, b, 0, stream>>>(a); break;
-    case 128: weights_kernel<kType, 128><<<g, b, 0, stream>>>(a); break;
-    default: weights_kernel<kType, 256><<<g, b, 0, stream>>>(a); break;
+constexpr int kFewWeightRows = 32;
+template <int kType, int kHd>
+hipError_t weights_typed(const WeightsArgs& a, hipStream_t stream) {
+  const int64_t pairs = (int64_t)a.batch.num_seqs * a.cache.heads;
+  if ((int64_t)a.batch.max_seqlen * a.per_kv <= kFewWeightRows) {
+    constexpr int kTiles = kHd == 256 ? 2 : 4, kKeys = kWaves * kTiles * 16;
+    const dim3 grid((unsigned)(pairs * ((a.width + kKeys - 1) / kKeys)));
+    weights_few_kernel<kType, kHd, kTiles><<<grid, dim3(kThreads), 0, stream>>>(a);
+  } else {
+    constexpr int kKeys = kWaves * 32;
+    const dim3 grid((unsigned)(pairs * ((a.width + kKeys - 1) / kKeys)));
+    weights_many_kernel<kType, kHd><<<grid, dim3(kThreads), 0, stream>>>(a);
   }
   return hipGetLastError();
+}
+
+template <int kType>
+hipError_t weights_sized(const WeightsArgs& a, hipStream_t stream) {
+  switch (padded_head(a.cache.head_dim)) {
+    case 64: return weights_typed<kType, 64>(a, stream);
+    case 128: return weights_typed<kType, 128>(a, stream);
+    default: return weights_typed<kType, 256>(a, stream);
+  }
 }
 
 }  // namespace
