@@ -20,6 +20,8 @@
 // rounded to bf16 for the second product. Where that product is not what bounds
 // the kernel (few query rows) or the query is fp16, the rounding's remainder is
 // added as a second bf16 operand, which leaves P with 16 bits.
+#include <type_traits>
+
 #include "kvx_step.h"
 
 namespace kvx {
@@ -438,8 +440,8 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 // Chunks of prompts: many query rows, bound by the matrix cores and the
 // softmax's VALU work beside them.
 //
-// A workgroup of four waves takes 4 * 32 * kCols query rows of one (sequence, KV
-// head) and passes over the keys kKeys at a time. The waves convert the codes
+// A workgroup takes 32 query rows a wave of one (sequence, KV head) and passes
+// over the keys kKeys at a time. The waves convert the codes
 // to bf16 (K: the query's type) into LDS once for all of them: K's rows as they
 // are, V transposed, with the exponent of its scale applied by the converting
 // instruction. LDS is double-buffered, the codes of the next keys are loaded
@@ -448,9 +450,8 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 // As above, S^T = K Q^T and O^T = V^T P^T, now by mfma 32x32x16: lane (n, h), n =
 // lane % 32, h = lane / 32, gets query row n's scores of keys 8 (i / 4) + 4 h + i % 4;
 // V^T's rows in LDS hold the keys in the order in which P lies in the lanes.
-// A wave's step is 32 keys: the scores of the next step, the softmax of this
-// one and the output of the one before it are independent of each other, so that
-// the matrix cores work under the softmax.
+// A wave's step is 32 keys: the scores of the next step are computed under the
+// exponentials of this one, and the other wave of the SIMD fills what is left.
 // The maximum that exponents are taken from moves only when a score exceeds it
 // by 2^8: P <= 2^8 costs bf16 and fp32 no precision, and most steps need neither
 // a reduction over lanes nor a pass over the outputs.
@@ -476,13 +477,21 @@ struct KeyInfo {
   float k_scale[kTiles16], v_scale[kTiles16];
 };
 
-template <int kType, int kHd, int kWaves, int kCols, int kKeys, int kParts>
+// `x`, which the compiler cannot tell from a new value: what is derived from it is computed where it is used, where it
+// would otherwise be kept in registers over whole loops that have none to spare.
+template <int kThreads>
+__device__ __forceinline__ unsigned recomputed(unsigned x) {
+  asm volatile("" : "+v"(x));
+  return x % kThreads;
+}
+
+template <int kType, int kHd, int kWaves, int kKeys, int kParts>
 __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
   using Q = Query<kType>;
   using T = typename Q::T;
   using Vec = typename Q::Vec;
   constexpr int kThreads = kWaves * kWave;
-  constexpr int kRows = 32 * kCols;           // of a wave
+  constexpr int kRows = 32;                   // of a wave
   constexpr int kSteps = kKeys / 32;
   constexpr int kTiles16 = kKeys / 16;
   constexpr int kDots = kHd / 16;             // mfmas over the head for 32 keys
@@ -523,15 +532,14 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     const int most = wave_last < first_row ? -1 : context - rows.count + (int)a.per_kv_of(wave_last);
     const int least = context - rows.count + (int)a.per_kv_of(first_row);
 
-    Vec q[kCols][kDots];
-    int last[kCols], out_row[kCols];
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      const int r = first_row + n * 32 + n32;
-      const bool real = r < num_rows;
-      const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
-      last[n] = real ? context - rows.count + nth : -1;
-      out_row[n] = real ? (rows.first + nth) * a.q_heads + head * a.per_kv + sub : -1;
+    Vec q[kDots];
+    const int r = first_row + n32;
+    const bool real = r < num_rows;
+    const int nth = a.per_kv_of(r), sub = r - nth * a.per_kv;
+    const int last = real ? context - rows.count + nth : -1;
+    const int out_row = real ? (rows.first + nth) * a.q_heads + head * a.per_kv + sub : -1;
+    {
+      const unsigned h = recomputed<kThreads>(threadIdx.x) % kWave / 32;
       const T* src = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride +
                      (int64_t)(head * a.per_kv + sub) * cache.head_dim;
 #pragma unroll
@@ -539,25 +547,18 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         const int at = d * 16 + h * 8;
         u32x4 w = {0, 0, 0, 0};
         if (real && at < cache.head_dim) w = *reinterpret_cast<const u32x4*>(src + at);
-        q[n][d] = __builtin_bit_cast(Vec, w);
+        q[d] = __builtin_bit_cast(Vec, w);
       }
     }
-    f32x16 o[kCols][kOuts];
-    float top[kCols], base[kCols], sum[kCols];
-    u32x4 p[kCols][2], p_low[kCols][2];
+    f32x16 o[kOuts];
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      top[n] = -INFINITY;
-      base[n] = sum[n] = 0.0f;
+    for (int d = 0; d < kOuts; ++d)
 #pragma unroll
-      for (int d = 0; d < kOuts; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][d][i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) p[n][i] = p_low[n][i] = u32x4{0, 0, 0, 0};
-    }
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float top = -INFINITY, base = 0.0f, sum = 0.0f;
 
     auto look_up = [&](int pass) {
+      const unsigned tid = recomputed<kThreads>(threadIdx.x);
       if (tid == 0) nan_steps[pass & 3] = 0;
       if (tid < kTiles16) {
         KeyInfo<kTiles16>& to = info[pass & 3];
@@ -572,7 +573,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
           }
         }
         to.row[tid] = row;
-        to.k_scale[tid] = row < 0 ? 0.0f : cache.k_scale[scale] * a.scale;
+        to.k_scale[tid] = row < 0 ? 1.0f : cache.k_scale[scale] * a.scale;
         to.v_scale[tid] = row < 0 ? 1.0f : cache.v_scale[scale];
       }
     };
@@ -580,20 +581,21 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     uint32_t v_raw[kVLoads][8][kVCols / 4];
     auto load = [&](int pass) {
       const KeyInfo<kTiles16>& from = info[pass & 3];
+      const unsigned tid = recomputed<kThreads>(threadIdx.x);
       constexpr int kPieces = kHd / 16;  // of a key's row
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        const int piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 16;
+        const unsigned piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 16;
         const int64_t row = from.row[key / 16];
         k_raw[i] = u32x4{0, 0, 0, 0};
-        if (row >= 0 && at < cache.head_dim)
+        if (row >= 0 && (int)at < cache.head_dim)
           k_raw[i] = *reinterpret_cast<const u32x4*>(cache.k + row * cache.head_dim + (key % 16) * row_bytes + at);
       }
 #pragma unroll
       for (int i = 0; i < kVLoads; ++i) {
-        const int group = (i * kThreads + tid) / kVThreads, at = tid % kVThreads * kVCols;
+        const unsigned group = (i * kThreads + tid) / kVThreads, at = tid % kVThreads * kVCols;
         const int64_t row = from.row[group / 2];
-        const bool there = row >= 0 && at < cache.head_dim;
+        const bool there = row >= 0 && (int)at < cache.head_dim;
         const uint8_t* src = cache.v + row * cache.head_dim + (group % 2) * 4 * row_bytes + at;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // keys 4 h + 0..3, then 8 + 4 h + 0..3
@@ -611,12 +613,13 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     };
     auto convert = [&](int pass) {
       const KeyInfo<kTiles16>& from = info[pass & 3];
+      const unsigned tid = recomputed<kThreads>(threadIdx.x);
       uint8_t* k_to = k_lds[pass & 1];
       uint8_t* v_to = v_lds[pass & 1];
       constexpr int kPieces = kHd / 16;
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        const int piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 32;
+        const unsigned piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 32;
         u32x4* to = reinterpret_cast<u32x4*>(k_to + key * kKRow + at);
         to[0] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].x, k_raw[i].y));
         to[1] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].z, k_raw[i].w));
@@ -624,7 +627,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       const bool masked = pass * kKeys + kKeys - 1 > group_least;  // some row does not see some key
 #pragma unroll
       for (int i = 0; i < kVLoads; ++i) {
-        const int group = (i * kThreads + tid) / kVThreads, col = tid % kVThreads * kVCols;
+        const unsigned group = (i * kThreads + tid) / kVThreads, col = tid % kVThreads * kVCols;
         const float scale = from.v_scale[group / 2];
         const float rest = scale / __uint_as_float(__float_as_uint(scale) & 0x7F800000u);
         if (masked) {
@@ -658,45 +661,101 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
                 w[j] = pack_bf16(__uint_as_float(w[j] << 16) * rest, __uint_as_float(w[j] & 0xFFFF0000u) * rest);
             }
             // The XOR spreads neighbouring threads' columns, kVCols rows apart, over the banks.
-            const int row = col + 4 * k + d;
+            const unsigned row = col + 4 * k + d;
             *reinterpret_cast<u32x4*>(v_to + row * kVRow + ((group ^ (row / 8 % 8)) * 16)) = w;
           }
         }
       }
     };
-    // S^T of 32 keys.
-    auto scores = [&](int buffer, int step, f32x16 (&s)[kCols]) {
-      const uint8_t* from = k_lds[buffer] + (step * 32 + n32) * kKRow + h * 16;
-#pragma unroll
-      for (int n = 0; n < kCols; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < kDots; ++d) {
-        const Vec k = *reinterpret_cast<const Vec*>(from + d * 32);
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) s[n] = mfma32<kType>(k, q[n][d], s[n]);
-      }
-    };
-    // O^T += V^T P^T of 32 keys. With the XOR above, a lane's row d * 32 + n32 holds the 8 keys 4 step + 2 i + h in the
-    // place (step ^ d) % 2 * 4 + (2 i + h ^ n32 / 8) of the 8 that step / 2 begins.
+    // S^T of a step's 32 keys: K's operand for columns 16 d .. is at k_at(step)[d * 32].
+    const int k_lane = n32 * kKRow + h * 16;
+    auto k_at = [&](int buffer, int step) { return k_lds[buffer] + step * 32 * kKRow + k_lane; };
+    // O^T += V^T P^T. With the XOR above, a lane's row d * 32 + n32 holds the 8 keys 4 step + 2 i + h in the place
+    // (step ^ d) % 2 * 4 + (2 i + h ^ n32 / 8) of the 8 that step / 2 begins.
     const int v_lane[2] = {n32 * kVRow + (h ^ (n32 / 8)) * 16, n32 * kVRow + ((2 + h) ^ (n32 / 8)) * 16};
-    auto add_outputs = [&](int buffer, int step) {
-      const uint8_t* from = v_lds[buffer] + step / 2 * 128;
+    auto v_at = [&](int buffer, int step, int i, int d) {
+      return v_lds[buffer] + step / 2 * 128 + (step + d) % 2 * 64 + v_lane[i] + d * 32 * kVRow;
+    };
+    // One step: the maximum, this step's P beside the scores of the next (kMore), which replace `x`, and this step's
+    // output. Operands are read kAhead products ahead. The scheduling barriers keep it so: left alone, the compiler
+    // waits for each operand right before its product.
+    auto work = [&](auto more, int pass, int step, f32x16& x) {
+      constexpr bool kMore = decltype(more)::value;
+      constexpr int kAhead = 2, kTurns = kDots, kEach = 8 / kTurns;
+      static_assert(kTurns == 2 * kOuts && kEach * kTurns == 8, "as many products in both");
+      const KeyInfo<kTiles16>& now = info[pass & 3];
+      const int buffer = pass & 1, key0 = pass * kKeys + step * 32;
+      const float scale[2] = {now.k_scale[step * 2], now.k_scale[step * 2 + 1]};
+      const bool there[2] = {now.row[step * 2] >= 0, now.row[step * 2 + 1] >= 0};
+      if (key0 + 31 > least || !there[0] || !there[1]) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint8_t* even = from + step % 2 * 64 + v_lane[i];
-        const uint8_t* odd = from + (1 - step % 2) * 64 + v_lane[i];
-#pragma unroll
-        for (int d = 0; d < kOuts; ++d) {
-          const bf16x8 v = *reinterpret_cast<const bf16x8*>((d % 2 ? odd : even) + d * 32 * kVRow);
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) {
-            o[n][d] = mfma32<KVX_DTYPE_BF16>(v, __builtin_bit_cast(bf16x8, p[n][i]), o[n][d]);
-            if (kParts > 1) o[n][d] = mfma32<KVX_DTYPE_BF16>(v, __builtin_bit_cast(bf16x8, p_low[n][i]), o[n][d]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          const bool see = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last && there[i / 8];
+          x[i] = see ? x[i] : -INFINITY;
         }
       }
+      float low = x[0], high = x[8];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        low = fmaxf(low, x[i]);
+        high = fmaxf(high, x[8 + i]);
+      }
+      high = fmaxf(low * scale[0], high * scale[1]);
+      if (__any(high > top + 8.0f)) {
+        top = fmaxf(top, fmaxf(high, __shfl_xor(high, 32)));
+        // A whole number, so that `fade` is a power of two and nothing is rounded.
+        const float now_base = top == -INFINITY ? base : ceilf(top);
+        const float fade = __builtin_amdgcn_exp2f(base - now_base);
+        base = now_base;
+        sum *= fade;
+#pragma unroll
+        for (int d = 0; d < kOuts; ++d) o[d] *= fade;
+      }
+      f32x16 next;
+      Vec k_next[kAhead + 1];
+      auto read_k = [&](int t) { k_next[t % (kAhead + 1)] = *reinterpret_cast<const Vec*>(k_at(buffer, step + 1) + t * 32); };
+      if (kMore) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) read_k(t);
+      }
+      u32x4 p[kParts][2];
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        if (kMore) {
+          if (t + kAhead < kTurns) read_k(t + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+          next = mfma32<kType>(k_next[t % (kAhead + 1)], q[t], next);
+        }
+#pragma unroll
+        for (int i = t * kEach; i < (t + 1) * kEach; ++i) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], scale[i / 4], -base));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], scale[i / 4], -base));
+          sum += e0 + e1;
+          const uint32_t hi = pack_bf16(e0, e1);
+          p[0][i / 4][i % 4] = hi;
+          if (kParts > 1)
+            p[kParts - 1][i / 4][i % 4] = pack_bf16(e0 - __uint_as_float(hi << 16), e1 - __uint_as_float(hi & 0xFFFF0000u));
+        }
+        if (kMore) __builtin_amdgcn_sched_barrier(0);
+      }
+      bf16x8 v_next[kAhead + 1];
+      auto read_v = [&](int t) {
+        v_next[t % (kAhead + 1)] = *reinterpret_cast<const bf16x8*>(v_at(buffer, step, t / kOuts, t % kOuts));
+      };
+#pragma unroll
+      for (int t = 0; t < kAhead; ++t) read_v(t);
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        if (t + kAhead < kTurns) read_v(t + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+          o[t % kOuts] = mfma32<KVX_DTYPE_BF16>(v_next[t % (kAhead + 1)], __builtin_bit_cast(bf16x8, p[k][t / kOuts]),
+                                               o[t % kOuts]);
+      }
+      if (kMore) x = next;
     };
 
     if (passes > first_pass) {
@@ -714,91 +773,18 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       if (pass + 1 < passes) load(pass + 1);
       const int steps = most < pass * kKeys ? 0 : min(kSteps, (most - pass * kKeys) / 32 + 1);
       if (steps > 0) {
-        f32x16 x[kCols], next[kCols];
-        scores(buffer, 0, x);
+        f32x16 x;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDots; ++d) x = mfma32<kType>(*reinterpret_cast<const Vec*>(k_at(buffer, 0) + d * 32), q[d], x);
 #pragma unroll 1
-        for (int step = 0; step < steps; ++step) {
-          {
-            const int key0 = pass * kKeys + step * 32;
-            const float scale[2] = {now.k_scale[step * 2], now.k_scale[step * 2 + 1]};
-            const bool there[2] = {now.row[step * 2] >= 0, now.row[step * 2 + 1] >= 0};
-            if (key0 + 31 > least || !there[0] || !there[1]) {
-#pragma unroll
-              for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const bool see = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last[n] && there[i / 8];
-                  x[n][i] = see ? x[n][i] * scale[i / 8] : -INFINITY;
-                }
-            } else {
-#pragma unroll
-              for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[n][i] *= scale[i / 8];
-            }
-            float high[kCols];
-            bool over = false;
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) {
-              high[n] = x[n][0];
-#pragma unroll
-              for (int i = 1; i < 16; ++i) high[n] = fmaxf(high[n], x[n][i]);
-              over = over || high[n] > top[n] + 8.0f;
-            }
-            if (__any(over)) {
-#pragma unroll
-              for (int n = 0; n < kCols; ++n) {
-                top[n] = fmaxf(top[n], fmaxf(high[n], __shfl_xor(high[n], 32)));
-                // A whole number, so that `fade` is a power of two and nothing is rounded.
-                const float now_base = top[n] == -INFINITY ? base[n] : ceilf(top[n]);
-                const float fade = __builtin_amdgcn_exp2f(base[n] - now_base);
-                base[n] = now_base;
-                sum[n] *= fade;
-#pragma unroll
-                for (int d = 0; d < kOuts; ++d) o[n][d] *= fade;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    p[n][i][j] = pack_bf16(__uint_as_float(p[n][i][j] << 16) * fade,
-                                           __uint_as_float(p[n][i][j] & 0xFFFF0000u) * fade);
-                    if (kParts > 1)
-                      p_low[n][i][j] = pack_bf16(__uint_as_float(p_low[n][i][j] << 16) * fade,
-                                                 __uint_as_float(p_low[n][i][j] & 0xFFFF0000u) * fade);
-                  }
-              }
-            }
-            scores(buffer, step + 1 < steps ? step + 1 : step, next);
-            add_outputs(buffer, step > 0 ? step - 1 : 0);
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) {
-              uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float e0 = __builtin_amdgcn_exp2f(x[n][2 * i] - base[n]);
-                const float e1 = __builtin_amdgcn_exp2f(x[n][2 * i + 1] - base[n]);
-                sum[n] += e0 + e1;
-                hi[i] = pack_bf16(e0, e1);
-                if (kParts > 1)
-                  lo[i] = pack_bf16(e0 - __uint_as_float(hi[i] << 16), e1 - __uint_as_float(hi[i] & 0xFFFF0000u));
-              }
-              p[n][0] = u32x4{hi[0], hi[1], hi[2], hi[3]};
-              p[n][1] = u32x4{hi[4], hi[5], hi[6], hi[7]};
-              if (kParts > 1) {
-                p_low[n][0] = u32x4{lo[0], lo[1], lo[2], lo[3]};
-                p_low[n][1] = u32x4{lo[4], lo[5], lo[6], lo[7]};
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) x[n] = next[n];
-          }
-        }
-        add_outputs(buffer, steps - 1);
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) p[n][0] = p[n][1] = p_low[n][0] = p_low[n][1] = u32x4{0, 0, 0, 0};
+        for (int step = 0; step < steps - 1; ++step) work(std::true_type{}, pass, step, x);
+        work(std::false_type{}, pass, steps - 1, x);
         const uint32_t nan = nan_steps[pass & 3];
         if (nan) {
           // Rows that see a NaN code in a pass that is masked for others: its columns become NaN.
+          const unsigned lane = recomputed<kThreads>(threadIdx.x) % kWave, n32 = lane % 32, h = lane / 32;
 #pragma unroll 1
           for (int step = 0; step < steps; ++step) {
             if (!(nan >> step & 1)) continue;
@@ -806,14 +792,12 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
             for (int i = 0; i < 2; ++i) {
               const int64_t row = now.row[step * 2 + i];
               if (row < 0) continue;
-              u32x4 seen[kCols];
+              u32x4 seen;
 #pragma unroll
-              for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int key = pass * kKeys + step * 32 + i * 16 + 4 * h + (j < 2 ? 2 * j : 4 + 2 * j);
-                  seen[n][j] = (key <= last[n] ? 0x3F80u : 0u) | (key + 1 <= last[n] ? 0x3F800000u : 0u);
-                }
+              for (int j = 0; j < 4; ++j) {
+                const int key = pass * kKeys + step * 32 + i * 16 + 4 * h + (j < 2 ? 2 * j : 4 + 2 * j);
+                seen[j] = (key <= last ? 0x3F80u : 0u) | (key + 1 <= last ? 0x3F800000u : 0u);
+              }
 #pragma unroll
               for (int d = 0; d < kOuts; ++d) {
                 const int col = d * 32 + n32;
@@ -826,15 +810,12 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
                     is_nan[j / 2] |= (code & 0x7F) == 0x7F ? (j % 2 ? 0x3F800000u : 0x3F80u) : 0u;
                   }
                 }
+                f32x16 hit;
 #pragma unroll
-                for (int n = 0; n < kCols; ++n) {
-                  f32x16 hit;
+                for (int j = 0; j < 16; ++j) hit[j] = 0.0f;
+                hit = mfma32<KVX_DTYPE_BF16>(__builtin_bit_cast(bf16x8, is_nan), __builtin_bit_cast(bf16x8, seen), hit);
 #pragma unroll
-                  for (int j = 0; j < 16; ++j) hit[j] = 0.0f;
-                  hit = mfma32<KVX_DTYPE_BF16>(__builtin_bit_cast(bf16x8, is_nan), __builtin_bit_cast(bf16x8, seen[n]), hit);
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) o[n][d][j] += hit[j] > 0.0f ? NAN : 0.0f;
-                }
+                for (int j = 0; j < 16; ++j) o[d][j] += hit[j] > 0.0f ? NAN : 0.0f;
               }
             }
           }
@@ -844,18 +825,17 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       __syncthreads();
     }
 
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      const float total = sum[n] + __shfl_xor(sum[n], 32);
-      if (out_row[n] < 0) continue;
+    const float total = sum + __shfl_xor(sum, 32);
+    if (out_row >= 0) {
+      const unsigned h = recomputed<kThreads>(threadIdx.x) % kWave / 32;
 #pragma unroll
       for (int d = 0; d < kOuts; ++d)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const int col = d * 32 + 8 * (i / 4) + 4 * h;
           if (col < cache.head_dim)
-            write_rows<T>(a, split, out_row[n], col, top[n] == -INFINITY ? -INFINITY : base[n], total,
-                          f32x4{o[n][d][i], o[n][d][i + 1], o[n][d][i + 2], o[n][d][i + 3]});
+            write_rows<T>(a, split, out_row, col, top == -INFINITY ? -INFINITY : base, total,
+                          f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]});
         }
     }
     __syncthreads();  // before the next rows' passes write to LDS
@@ -1245,7 +1225,7 @@ hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
   } else {
     if constexpr (kHd < 256) {
       const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles;
-      chunk_kernel<kType, kHd, kChunkWaves, 1, chunk_keys(kHd), kType == KVX_DTYPE_BF16 ? 1 : 2>
+      chunk_kernel<kType, kHd, kChunkWaves, chunk_keys(kHd), kType == KVX_DTYPE_BF16 ? 1 : 2>
           <<<dim3((unsigned)grid), dim3(kChunkWaves * kWave), 0, stream>>>(a);
       err = hipGetLastError();
     } else {
