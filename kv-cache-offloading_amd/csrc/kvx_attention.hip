@@ -92,6 +92,25 @@ __device__ __forceinline__ void transpose4(const uint32_t* x, uint32_t* out) {
   out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
+// A value that all lanes have, in a scalar register.
+__device__ __forceinline__ int64_t scalar(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float scalar(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+}
+// A lane's value, in a scalar register.
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0x80 in each byte that is a NaN code
   return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
@@ -499,7 +518,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
   constexpr int kKRow = kHd * 2 + 16;         // bytes between rows in LDS: 16 more, so that 8 lanes' pieces meet no bank twice
   constexpr int kVRow = kKeys * 2 + 16;
   constexpr int kKLoads = kKeys * kHd / 16 / kThreads;  // 16-byte pieces of K a thread
-  constexpr int kVCols = kWaves == 4 && kHd > 64 ? 8 : 4;  // adjacent columns of V that a thread transposes
+  constexpr int kVCols = 4;                             // adjacent columns of V that a thread transposes
   constexpr int kVThreads = kHd / kVCols;               // for a group of 8 keys
   constexpr int kVLoads = kKeys / 8 * kVThreads / kThreads;
   static_assert(kKLoads * kThreads * 16 == kKeys * kHd && kVLoads * kThreads == kKeys / 8 * kVThreads, "whole pieces");
@@ -557,113 +576,115 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float top = -INFINITY, base = 0.0f, sum = 0.0f;
 
-    auto look_up = [&](int pass) {
+    // The lookup of a pass's tiles by the first lanes: its blocks two passes before they are needed in LDS, their scales
+    // one, so that neither load is waited for.
+    int block_id = -1;
+    int64_t found_row = -1;
+    float found_k = 1.0f, found_v = 1.0f;
+    auto find_block = [&](int pass) {
+      const unsigned tid = recomputed<kThreads>(threadIdx.x);
+      const int key = pass * kKeys + (int)tid * 16;
+      block_id = tid < kTiles16 && key < context ? table[cache.block_of(key)] : -1;
+    };
+    auto find_scales = [&](int pass) {
+      const unsigned tid = recomputed<kThreads>(threadIdx.x);
+      const int key = pass * kKeys + (int)tid * 16;
+      found_row = -1;
+      found_k = found_v = 1.0f;
+      if (block_id >= 0 && block_id < cache.num_blocks) {
+        const int in = key - cache.block_of(key) * cache.block_size;
+        const int64_t at = ((int64_t)block_id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head;
+        found_row = ((int64_t)block_id * cache.block_size + in) * cache.heads + head;
+        found_k = cache.k_scale[at];
+        found_v = cache.v_scale[at];
+      }
+    };
+    auto put_info = [&](int pass) {
       const unsigned tid = recomputed<kThreads>(threadIdx.x);
       if (tid == 0) nan_steps[pass & 3] = 0;
       if (tid < kTiles16) {
-        KeyInfo<kTiles16>& to = info[pass & 3];
-        const int key = pass * kKeys + tid * 16;
-        int64_t row = -1, scale = 0;
-        if (key < context) {
-          const int nth = cache.block_of(key), in = key - nth * cache.block_size;
-          const int id = table[nth];
-          if (id >= 0 && id < cache.num_blocks) {
-            row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
-            scale = ((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head;
-          }
-        }
-        to.row[tid] = row;
-        to.k_scale[tid] = row < 0 ? 1.0f : cache.k_scale[scale] * a.scale;
-        to.v_scale[tid] = row < 0 ? 1.0f : cache.v_scale[scale];
+        info[pass & 3].row[tid] = found_row;
+        info[pass & 3].k_scale[tid] = found_row < 0 ? 1.0f : found_k * a.scale;
+        info[pass & 3].v_scale[tid] = found_v;
       }
     };
     u32x4 k_raw[kKLoads];
-    uint32_t v_raw[kVLoads][8][kVCols / 4];
+    uint32_t v_raw[kVLoads][8];
+    // Where a wave's lanes all read one 16-key tile, its address and scale are scalars.
+    constexpr int kPieces = kHd / 16;  // of a key's row
+    static_assert(kWave / kPieces <= 16 && 16 % (kWave / kPieces) == 0, "a wave's pieces of K lie in one tile");
+    constexpr bool kVUniform = kVThreads * 2 >= kWave;
     auto load = [&](int pass) {
       const KeyInfo<kTiles16>& from = info[pass & 3];
-      const unsigned tid = recomputed<kThreads>(threadIdx.x);
-      constexpr int kPieces = kHd / 16;  // of a key's row
+      const unsigned lane = recomputed<kThreads>(threadIdx.x) % kWave;
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        const unsigned piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 16;
-        const int64_t row = from.row[key / 16];
+        const int key = (i * kThreads + wave * kWave) / kPieces;  // the wave's first
+        const unsigned at = lane % kPieces * 16;
+        const int64_t row = scalar(from.row[key / 16]);
+        const uint8_t* tile = cache.k + row * cache.head_dim + key % 16 * row_bytes;
         k_raw[i] = u32x4{0, 0, 0, 0};
         if (row >= 0 && (int)at < cache.head_dim)
-          k_raw[i] = *reinterpret_cast<const u32x4*>(cache.k + row * cache.head_dim + (key % 16) * row_bytes + at);
+          k_raw[i] = *reinterpret_cast<const u32x4*>(tile + (lane / kPieces * (unsigned)row_bytes + at));
       }
 #pragma unroll
       for (int i = 0; i < kVLoads; ++i) {
-        const unsigned group = (i * kThreads + tid) / kVThreads, at = tid % kVThreads * kVCols;
-        const int64_t row = from.row[group / 2];
+        const unsigned group = (i * kThreads + wave * kWave + lane) / kVThreads, at = lane % kVThreads * kVCols;
+        const int64_t row = kVUniform ? scalar(from.row[(i * kThreads + wave * kWave) / kVThreads / 2]) : from.row[group / 2];
         const bool there = row >= 0 && (int)at < cache.head_dim;
-        const uint8_t* src = cache.v + row * cache.head_dim + (group % 2) * 4 * row_bytes + at;
+        const uint8_t* tile = cache.v + row * cache.head_dim;
+        const unsigned in_tile = group % 2 * 4 * (unsigned)row_bytes + at;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // keys 4 h + 0..3, then 8 + 4 h + 0..3
-          const uint8_t* from_row = src + (j < 4 ? j : j + 4) * row_bytes;
-          if constexpr (kVCols == 4) {
-            v_raw[i][j][0] = there ? *reinterpret_cast<const uint32_t*>(from_row) : 0;
-          } else {
-            u32x2 w = {0, 0};
-            if (there) w = *reinterpret_cast<const u32x2*>(from_row);
-            v_raw[i][j][0] = w.x;
-            v_raw[i][j][1] = w.y;
-          }
+          v_raw[i][j] = 0;
+          if (there) v_raw[i][j] = *reinterpret_cast<const uint32_t*>(tile + (j < 4 ? j : j + 4) * row_bytes + in_tile);
         }
       }
     };
     auto convert = [&](int pass) {
       const KeyInfo<kTiles16>& from = info[pass & 3];
-      const unsigned tid = recomputed<kThreads>(threadIdx.x);
+      const unsigned lane = recomputed<kThreads>(threadIdx.x) % kWave;
       uint8_t* k_to = k_lds[pass & 1];
       uint8_t* v_to = v_lds[pass & 1];
-      constexpr int kPieces = kHd / 16;
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        const unsigned piece = i * kThreads + tid, key = piece / kPieces, at = piece % kPieces * 32;
-        u32x4* to = reinterpret_cast<u32x4*>(k_to + key * kKRow + at);
+        const int key = (i * kThreads + wave * kWave) / kPieces;
+        u32x4* to = reinterpret_cast<u32x4*>(k_to + key * kKRow + (lane / kPieces * kKRow + lane % kPieces * 32));
         to[0] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].x, k_raw[i].y));
         to[1] = __builtin_bit_cast(u32x4, decode8<Q>(k_raw[i].z, k_raw[i].w));
       }
       const bool masked = pass * kKeys + kKeys - 1 > group_least;  // some row does not see some key
 #pragma unroll
       for (int i = 0; i < kVLoads; ++i) {
-        const unsigned group = (i * kThreads + tid) / kVThreads, col = tid % kVThreads * kVCols;
-        const float scale = from.v_scale[group / 2];
-        const float rest = scale / __uint_as_float(__float_as_uint(scale) & 0x7F800000u);
+        const unsigned group = (i * kThreads + wave * kWave + lane) / kVThreads, col = lane % kVThreads * kVCols;
+        const float scale = kVUniform ? scalar(from.v_scale[(i * kThreads + wave * kWave) / kVThreads / 2]) : from.v_scale[group / 2];
+        const float rest = __uint_as_float((__float_as_uint(scale) & 0x007FFFFFu) | 0x3F800000u);  // in [1, 2)
         if (masked) {
           uint32_t nan = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int k = 0; k < kVCols / 4; ++k) nan |= nan_bytes(v_raw[i][j][k]);
+          for (int j = 0; j < 8; ++j) nan |= nan_bytes(v_raw[i][j]);
           if (nan) {
             atomicOr(&nan_steps[pass & 3], 1u << (group / 4));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-              for (int k = 0; k < kVCols / 4; ++k) v_raw[i][j][k] &= ~((nan_bytes(v_raw[i][j][k]) >> 7) * 0xFFu);
+            for (int j = 0; j < 8; ++j) v_raw[i][j] &= ~((nan_bytes(v_raw[i][j]) >> 7) * 0xFFu);
           }
         }
+        uint32_t lo[4], hi[4];
+        transpose4(v_raw[i], lo);
+        transpose4(v_raw[i] + 4, hi);
+        // Column col + d is row col + d of V^T; as col is a multiple of 4, all four have the same row / 8. The XOR spreads
+        // neighbouring threads' columns, 4 rows apart, over the banks.
+        uint8_t* to = v_to + col * kVRow + ((group ^ (col / 8 % 8)) * 16);
 #pragma unroll
-        for (int k = 0; k < kVCols / 4; ++k) {
-          uint32_t in[8], lo[4], hi[4];
+        for (int d = 0; d < 4; ++d) {
+          u32x4 w = {pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
+                     pair_scaled(hi[d], scale, false), pair_scaled(hi[d], scale, true)};
+          if (rest != 1.0f) {  // no power of two: the rest of the scale costs V one rounding to bf16
 #pragma unroll
-          for (int j = 0; j < 8; ++j) in[j] = v_raw[i][j][k];
-          transpose4(in, lo);
-          transpose4(in + 4, hi);
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            u32x4 w = {pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
-                       pair_scaled(hi[d], scale, false), pair_scaled(hi[d], scale, true)};
-            if (rest != 1.0f) {  // no power of two: the rest of the scale costs V one rounding to bf16
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w[j] = pack_bf16(__uint_as_float(w[j] << 16) * rest, __uint_as_float(w[j] & 0xFFFF0000u) * rest);
-            }
-            // The XOR spreads neighbouring threads' columns, kVCols rows apart, over the banks.
-            const unsigned row = col + 4 * k + d;
-            *reinterpret_cast<u32x4*>(v_to + row * kVRow + ((group ^ (row / 8 % 8)) * 16)) = w;
+            for (int j = 0; j < 4; ++j)
+              w[j] = pack_bf16(__uint_as_float(w[j] << 16) * rest, __uint_as_float(w[j] & 0xFFFF0000u) * rest);
           }
+          *reinterpret_cast<u32x4*>(to + d * kVRow) = w;
         }
       }
     };
@@ -679,14 +700,20 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     // One step: the maximum, this step's P beside the scores of the next (kMore), which replace `x`, and this step's
     // output. Operands are read kAhead products ahead. The scheduling barriers keep it so: left alone, the compiler
     // waits for each operand right before its product.
+    float tile_scale = 0.0f;   // lane l: of the pass's tile l
+    uint32_t tiles_there = 0;  // bit l: whether tile l is in a block
+    constexpr int kAhead = 2;
+    Vec k_next[kAhead + 1];
+    auto read_k = [&](int buffer, int step, int t) {
+      k_next[t % (kAhead + 1)] = *reinterpret_cast<const Vec*>(k_at(buffer, step) + t * 32);
+    };
     auto work = [&](auto more, int pass, int step, f32x16& x) {
       constexpr bool kMore = decltype(more)::value;
-      constexpr int kAhead = 2, kTurns = kDots, kEach = 8 / kTurns;
+      constexpr int kTurns = kDots, kEach = 8 / kTurns;
       static_assert(kTurns == 2 * kOuts && kEach * kTurns == 8, "as many products in both");
-      const KeyInfo<kTiles16>& now = info[pass & 3];
       const int buffer = pass & 1, key0 = pass * kKeys + step * 32;
-      const float scale[2] = {now.k_scale[step * 2], now.k_scale[step * 2 + 1]};
-      const bool there[2] = {now.row[step * 2] >= 0, now.row[step * 2 + 1] >= 0};
+      const float scale[2] = {lane_value(tile_scale, step * 2), lane_value(tile_scale, step * 2 + 1)};
+      const bool there[2] = {(tiles_there >> (step * 2) & 1) != 0, (tiles_there >> (step * 2 + 1) & 1) != 0};
       if (key0 + 31 > least || !there[0] || !there[1]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -712,19 +739,23 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         for (int d = 0; d < kOuts; ++d) o[d] *= fade;
       }
       f32x16 next;
-      Vec k_next[kAhead + 1];
-      auto read_k = [&](int t) { k_next[t % (kAhead + 1)] = *reinterpret_cast<const Vec*>(k_at(buffer, step + 1) + t * 32); };
       if (kMore) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[i] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < kAhead; ++t) read_k(t);
       }
+      bf16x8 v_next[kAhead + 1];
+      auto read_v = [&](int t) {
+        v_next[t % (kAhead + 1)] = *reinterpret_cast<const bf16x8*>(v_at(buffer, step, t / kOuts, t % kOuts));
+      };
       u32x4 p[kParts][2];
+      // The wave that has scores and exponentials to issue goes first, so that the SIMD's two waves fall out of step and
+      // one's outputs run under the other's exponentials: 477 us in place of 511 for two chunks behind 6-8 K tokens.
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < kTurns; ++t) {
         if (kMore) {
-          if (t + kAhead < kTurns) read_k(t + kAhead);
+          if (t + kAhead < kTurns) read_k(buffer, step + 1, t + kAhead);
+          else read_v(t + kAhead - kTurns);
           __builtin_amdgcn_sched_barrier(0);
           next = mfma32<kType>(k_next[t % (kAhead + 1)], q[t], next);
         }
@@ -740,15 +771,15 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         }
         if (kMore) __builtin_amdgcn_sched_barrier(0);
       }
-      bf16x8 v_next[kAhead + 1];
-      auto read_v = [&](int t) {
-        v_next[t % (kAhead + 1)] = *reinterpret_cast<const bf16x8*>(v_at(buffer, step, t / kOuts, t % kOuts));
-      };
+      if (!kMore) {
 #pragma unroll
-      for (int t = 0; t < kAhead; ++t) read_v(t);
+        for (int t = 0; t < kAhead; ++t) read_v(t);
+      }
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int t = 0; t < kTurns; ++t) {
         if (t + kAhead < kTurns) read_v(t + kAhead);
+        else if (kMore) read_k(buffer, step + 2 < kSteps ? step + 2 : step, t + kAhead - kTurns);  // for the step after, if any
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < kParts; ++k)
@@ -759,8 +790,13 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     };
 
     if (passes > first_pass) {
-      look_up(first_pass);
-      look_up(first_pass + 1);
+      find_block(first_pass);
+      find_scales(first_pass);
+      put_info(first_pass);
+      find_block(first_pass + 1);
+      find_scales(first_pass + 1);
+      put_info(first_pass + 1);
+      find_block(first_pass + 2);
       __syncthreads();
       load(first_pass);
       convert(first_pass);
@@ -769,7 +805,8 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     for (int pass = first_pass; pass < passes; ++pass) {
       const int buffer = pass & 1;
       const KeyInfo<kTiles16>& now = info[pass & 3];
-      look_up(pass + 2);
+      find_scales(pass + 2);
+      find_block(pass + 3);
       if (pass + 1 < passes) load(pass + 1);
       const int steps = most < pass * kKeys ? 0 : min(kSteps, (most - pass * kKeys) / 32 + 1);
       if (steps > 0) {
@@ -778,6 +815,10 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         for (int i = 0; i < 16; ++i) x[i] = 0.0f;
 #pragma unroll
         for (int d = 0; d < kDots; ++d) x = mfma32<kType>(*reinterpret_cast<const Vec*>(k_at(buffer, 0) + d * 32), q[d], x);
+        tile_scale = now.k_scale[lane % kTiles16];
+        tiles_there = (uint32_t)__ballot(now.row[lane % kTiles16] >= 0);
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) read_k(buffer, 1, t);
 #pragma unroll 1
         for (int step = 0; step < steps - 1; ++step) work(std::true_type{}, pass, step, x);
         work(std::false_type{}, pass, steps - 1, x);
@@ -822,6 +863,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         }
       }
       if (pass + 1 < passes) convert(pass + 1);
+      put_info(pass + 2);
       __syncthreads();
     }
 
@@ -944,15 +986,6 @@ __device__ __forceinline__ KeyTile key_tile(const WeightsArgs& a, const int32_t*
   }
   return t;
 }
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane);
-  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ float lane_value(float x, int lane) {
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
-}
-
 // The sum over the 16 lanes of a row, in all of them.
 __device__ __forceinline__ float sum16(float x) {
   x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));  // row_ror:8
