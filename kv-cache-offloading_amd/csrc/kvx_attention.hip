@@ -672,9 +672,10 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         uint32_t lo[4], hi[4];
         transpose4(v_raw[i], lo);
         transpose4(v_raw[i] + 4, hi);
-        // Column col + d is row col + d of V^T; as col is a multiple of 4, all four have the same row / 8. The XOR spreads
-        // neighbouring threads' columns, 4 rows apart, over the banks.
-        uint8_t* to = v_to + col * kVRow + ((group ^ (col / 8 % 8)) * 16);
+        // Column col + d is row col + d of V^T; as col is a multiple of 4, all four have the same row / 16. The XOR spreads
+        // neighbouring threads' columns, 4 rows apart, over the banks, and leaves 16 lanes that read adjacent rows on
+        // banks of their own.
+        uint8_t* to = v_to + col * kVRow + ((group ^ (col / 16 % 4)) * 16);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           u32x4 w = {pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
@@ -691,11 +692,11 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     // S^T of a step's 32 keys: K's operand for columns 16 d .. is at k_at(step)[d * 32].
     const int k_lane = n32 * kKRow + h * 16;
     auto k_at = [&](int buffer, int step) { return k_lds[buffer] + step * 32 * kKRow + k_lane; };
-    // O^T += V^T P^T. With the XOR above, a lane's row d * 32 + n32 holds the 8 keys 4 step + 2 i + h in the place
-    // (step ^ d) % 2 * 4 + (2 i + h ^ n32 / 8) of the 8 that step / 2 begins.
-    const int v_lane[2] = {n32 * kVRow + (h ^ (n32 / 8)) * 16, n32 * kVRow + ((2 + h) ^ (n32 / 8)) * 16};
+    // O^T += V^T P^T. A lane's row d * 32 + n32 holds, of a step's four groups of 8 keys, group 2 i + h in place
+    // (2 i + h) ^ (row / 16 % 4).
+    const int v_lane = n32 * kVRow + (h ^ (n32 / 16)) * 16;
     auto v_at = [&](int buffer, int step, int i, int d) {
-      return v_lds[buffer] + step / 2 * 128 + (step + d) % 2 * 64 + v_lane[i] + d * 32 * kVRow;
+      return v_lds[buffer] + v_lane + step * 64 + (i ^ (d % 2)) * 32 + d * 32 * kVRow;
     };
     // One step: the maximum, this step's P beside the scores of the next (kMore), which replace `x`, and this step's
     // output. Operands are read kAhead products ahead. The scheduling barriers keep it so: left alone, the compiler
