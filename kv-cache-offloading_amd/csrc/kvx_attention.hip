@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
   const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
   const int tile = rest % a.row_tiles, split = rest / a.row_tiles;
   const int seq = pair / cache.heads, head = pair % cache.heads;
-  const int context = context_of(a.batch, seq, cache.block_size);
+  const int context = cache.num_blocks > 0 ? context_of(a.batch, seq, cache.block_size) : 0;
   const int first_step = split * a.split_steps;
   // The first split also writes the rows that see nothing.
   if (first_step * kStep >= context && split > 0) return;
@@ -172,7 +172,12 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
   const int num_rows = rows.count * a.per_kv;
   const int32_t* table = a.batch.tables + seq * a.batch.table_stride;
   const int64_t row_bytes = (int64_t)cache.heads * cache.head_dim;
-  const int32_t k_lane = c * (int32_t)row_bytes + g * 16, v_lane = 4 * g * (int32_t)row_bytes + c * kCols;
+  // A lane's places in a tile of K, 64 columns apart, and in one of V, a row apart. Columns past head_dim are read as
+  // others before it: the query is 0 there, and the output is not written.
+  uint32_t k_lane[kChunks];
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) k_lane[k] = c * (uint32_t)row_bytes + min(k * 64 + g * 16, cache.head_dim - 16);
+  const uint32_t v_lane = 4 * g * (uint32_t)row_bytes + min(c * kCols, cache.head_dim - kCols);
 
   // A launch covers max_seqlen queries a sequence; longer ones wrap around.
   for (int tile_row = tile * kRows; tile_row < num_rows; tile_row += a.row_tiles * kRows) {
@@ -217,10 +222,8 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
     const int my_first = first_step + wave;
     const int my_steps = my_first < end_step ? (end_step - my_first + kWaves - 1) / kWaves : 0;
 
-    struct Codes {
-      u32x4 k[2][kChunks];
-      uint32_t v[8][kCols / 4];
-    };
+    u32x4 k_codes[2][kChunks];
+    uint32_t v_codes[8][kCols / 4];
     int64_t info_row = -1;  // of tile lane % 2 of the batch's step lane / 2
     float info_k = 0.0f, info_v = 0.0f;
     auto look_up = [&](int nth) {
@@ -238,41 +241,37 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         }
       }
     };
-    auto row_of = [&](int nth, int t) {
-      const int at = nth % 32 * 2 + t;
-      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)info_row, at);
-      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(info_row >> 32), at);
-      return (int64_t)((uint64_t)hi << 32 | lo);
-    };
-    auto load = [&](int nth, Codes& to) {
+    auto row_of = [&](int nth, int t) { return lane_value(info_row, nth % 32 * 2 + t); };
+    // Loads without a condition (tiles that are not there read as the pool's first one, and count for nothing): behind
+    // one, the compiler would wait for all loads under way before it uses any.
+    // K: lane (c, g) takes columns 16 g .. 16 g + 15 of each 64 of key c's row.
+    auto load_k = [&](int nth) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int64_t row = row_of(nth, t);
-        // K: lane (c, g) takes columns 16 g .. 16 g + 15 of each 64 of key c's row.
-        const uint8_t* k_from = cache.k + row * cache.head_dim;
+        const uint8_t* tile = cache.k + (row < 0 ? 0 : row) * cache.head_dim;
 #pragma unroll
-        for (int k = 0; k < kChunks; ++k) {
-          to.k[t][k] = u32x4{0, 0, 0, 0};
-          if (row >= 0 && k * 64 + g * 16 < cache.head_dim)
-            to.k[t][k] = *reinterpret_cast<const u32x4*>(k_from + (k_lane + k * 64));
-        }
-        // V: columns kCols c .. of keys 4 g + i.
-        const uint8_t* v_from = cache.v + row * cache.head_dim;
-        const bool there = row >= 0 && c * kCols < cache.head_dim;
+        for (int k = 0; k < kChunks; ++k) k_codes[t][k] = *reinterpret_cast<const u32x4*>(tile + k_lane[k]);
+      }
+    };
+    // V: columns kCols c .. of keys 4 g + i.
+    auto load_v = [&](int nth) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int64_t row = row_of(nth, t);
+        const uint8_t* tile = cache.v + (row < 0 ? 0 : row) * cache.head_dim;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* p = v_from + (v_lane + i * (int32_t)row_bytes);
-          uint32_t(&v)[kCols / 4] = to.v[4 * t + i];
+          const uint8_t* p = tile + i * row_bytes + v_lane;
+          uint32_t(&v)[kCols / 4] = v_codes[4 * t + i];
           if constexpr (kCols == 4) {
-            v[0] = there ? *reinterpret_cast<const uint32_t*>(p) : 0;
+            v[0] = *reinterpret_cast<const uint32_t*>(p);
           } else if constexpr (kCols == 8) {
-            u32x2 w = {0, 0};
-            if (there) w = *reinterpret_cast<const u32x2*>(p);
+            const u32x2 w = *reinterpret_cast<const u32x2*>(p);
             v[0] = w.x;
             v[1] = w.y;
           } else {
-            u32x4 w = {0, 0, 0, 0};
-            if (there) w = *reinterpret_cast<const u32x4*>(p);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(p);
             v[0] = w.x;
             v[1] = w.y;
             v[2] = w.z;
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         }
       }
     };
-    auto use = [&](int nth, const Codes& codes) {
+    auto use = [&](int nth) {
       const int key0 = (my_first + nth * kWaves) * kStep;
       bool there[2];
       float ks[2], vs[2];
@@ -289,8 +288,8 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
       for (int t = 0; t < 2; ++t) {
         const int at = nth % 32 * 2 + t;
         there[t] = row_of(nth, t) >= 0;
-        ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(info_k), at));
-        vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_int(info_v), at));
+        ks[t] = lane_value(info_k, at);
+        vs[t] = lane_value(info_v, at);
       }
       f32x4 s[kTiles][2];
 #pragma unroll
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         for (int n = 0; n < kTiles; ++n) s[n][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-          const u32x4 w = codes.k[t][k];
+          const u32x4 w = k_codes[t][k];
           const Vec lo = decode8<Q>(w.x, w.y), hi = decode8<Q>(w.z, w.w);
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
@@ -308,6 +307,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
           }
         }
       }
+      load_k(nth + 1);
       // Keys that some row may not see, and codes in their places that are no numbers.
       const bool partial = key0 + kStep - 1 > least || !there[0] || !there[1];
       bool mend = false;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int k = 0; k < kCols / 4; ++k) nan |= nan_bytes(codes.v[j][k]);
+          for (int k = 0; k < kCols / 4; ++k) nan |= nan_bytes(v_codes[j][k]);
         mend = __any(nan != 0);
       }
       u32x4 p_hi[kTiles], p_lo[kTiles];
@@ -364,23 +364,23 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         p_hi[n] = u32x4{hi[0], hi[1], hi[2], hi[3]};
         p_lo[n] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
+      if (mend) {
+        // A key that is masked for a row adds nothing to it, though its code be NaN: NaN codes count as zeros, and rows
+        // that see one become NaN.
 #pragma unroll
-      for (int k = 0; k < kCols / 4; ++k) {
-        uint32_t in[8], lo[4], hi[4];
+        for (int k = 0; k < kCols / 4; ++k) {
+          uint32_t in[8], lo[4], hi[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) in[j] = codes.v[j][k];
-        transpose4(in, lo);
-        transpose4(in + 4, hi);
+          for (int j = 0; j < 8; ++j) {
+            in[j] = nan_bytes(v_codes[j][k]) >> 7;
+            v_codes[j][k] &= ~(in[j] * 0xFFu);
+            in[j] *= 0x38u;  // 1.0
+          }
+          transpose4(in, lo);
+          transpose4(in + 4, hi);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          uint32_t l = lo[d], h = hi[d];
-          if (mend) {
-            // A key that is masked for a row adds nothing to it, though its code be NaN: NaN codes
-            // count as zeros, and rows that see one become NaN.
-            const uint32_t l_nan = nan_bytes(l) >> 7, h_nan = nan_bytes(h) >> 7;
-            l &= ~(l_nan * 0xFFu);
-            h &= ~(h_nan * 0xFFu);
-            const bf16x8 is_nan = decode8<B>(l_nan * 0x38u, h_nan * 0x38u);  // 0x38: 1.0
+          for (int d = 0; d < 4; ++d) {
+            const bf16x8 is_nan = decode8<B>(lo[d], hi[d]);
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
               u32x4 w;
@@ -392,7 +392,18 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
               for (int i = 0; i < 4; ++i) o[n][4 * k + d][i] += hit[i] > 0.0f ? NAN : 0.0f;
             }
           }
-          const bf16x8 w = decode8<B>(l, h);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kCols / 4; ++k) {
+        uint32_t in[8], lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) in[j] = v_codes[j][k];
+        transpose4(in, lo);
+        transpose4(in + 4, hi);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const bf16x8 w = decode8<B>(lo[d], hi[d]);
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
             o[n][4 * k + d] = B::mfma(w, __builtin_bit_cast(bf16x8, p_hi[n]), o[n][4 * k + d]);
@@ -401,16 +412,17 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         }
       }
     };
-    Codes now, next;
-    for (int nth = 0; nth < my_steps; ++nth) {
-      if (nth % 32 == 0) {  // a new batch of steps
-        look_up(nth);
-        load(nth, now);
+    // K's registers are loaded for the next step once the scores are taken, V's once the outputs are; behind the last
+    // step, from some tile of the batch, for nothing.
+    for (int batch = 0; batch < my_steps; batch += 32) {
+      look_up(batch);
+      const int batch_end = min(batch + 32, my_steps);
+      load_k(batch);
+      load_v(batch);
+      for (int nth = batch; nth < batch_end; ++nth) {
+        use(nth);
+        load_v(nth + 1);
       }
-      const bool more = nth + 1 < my_steps && (nth + 1) % 32;
-      if (more) load(nth + 1, next);
-      use(nth, now);
-      if (more) now = next;
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
