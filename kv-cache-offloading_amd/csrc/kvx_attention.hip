@@ -158,12 +158,10 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
-  // Workgroup -> (sequence, KV head), query tile, split. Neighbouring
-  // workgroups take different heads, so that an XCD keeps to few of them.
-  const int pairs = a.batch.num_seqs * cache.heads;
-  const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+  const Slice slice = slice_of(blockIdx.x, cache.heads);
+  const int seq = slice.unit % a.batch.num_seqs, rest = slice.unit / a.batch.num_seqs, head = slice.head;
   const int tile = rest % a.row_tiles, split = rest / a.row_tiles;
-  const int seq = pair / cache.heads, head = pair % cache.heads;
+  if (split >= a.splits) return;
   const int context = cache.num_blocks > 0 ? context_of(a.batch, seq, cache.block_size) : 0;
   const int first_step = split * a.split_steps;
   // The first split also writes the rows that see nothing.
@@ -1018,9 +1016,9 @@ __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
   const Fp8Cache& cache = a.cache;
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int pairs = a.batch.num_seqs * cache.heads;
-  const int pair = blockIdx.x % pairs, seq = pair / cache.heads, head = pair % cache.heads;
-  const int key0 = ((blockIdx.x / pairs) * kWaves + wave) * kTiles * 16;
+  const Slice slice = slice_of(blockIdx.x, cache.heads);
+  const int seq = slice.unit % a.batch.num_seqs, head = slice.head, pair = seq * cache.heads + head;
+  const int key0 = (slice.unit / a.batch.num_seqs * kWaves + wave) * kTiles * 16;
   if (key0 >= a.width) return;
   const int context = context_of(a.batch, seq, cache.block_size);
   const int64_t base = (int64_t)pair * a.width;
@@ -1252,7 +1250,7 @@ constexpr int chunk_keys(int padded) { return 16384 / padded; }
 
 template <int kType, int kHd, int kTiles>
 hipError_t few_rows_of(const AttentionArgs& a, hipStream_t stream) {
-  const int64_t grid = (int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles;
+  const int64_t grid = slices_grid((int64_t)a.batch.num_seqs * a.splits * a.row_tiles, a.cache.heads);
   few_rows_kernel<kType, kHd, kTiles><<<dim3((unsigned)grid), dim3(kThreads), 0, stream>>>(a);
   return hipGetLastError();
 }
@@ -1299,7 +1297,7 @@ hipError_t weights_typed(const WeightsArgs& a, hipStream_t stream) {
   const int64_t pairs = (int64_t)a.batch.num_seqs * a.cache.heads;
   if ((int64_t)a.batch.max_seqlen * a.per_kv <= kFewWeightRows) {
     constexpr int kTiles = kHd == 256 ? 2 : 4, kKeys = kWaves * kTiles * 16;
-    const dim3 grid((unsigned)(pairs * ((a.width + kKeys - 1) / kKeys)));
+    const dim3 grid((unsigned)slices_grid((int64_t)a.batch.num_seqs * ((a.width + kKeys - 1) / kKeys), a.cache.heads));
     weights_few_kernel<kType, kHd, kTiles><<<grid, dim3(kThreads), 0, stream>>>(a);
   } else {
     constexpr int kKeys = kWaves * 32;

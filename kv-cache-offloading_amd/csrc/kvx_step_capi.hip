@@ -167,7 +167,8 @@ int kvx_store_kvcache_fp8(const kvx_fp8_cache* cache, const void* key, int64_t k
   if (num_tokens < 0) return set_error(KVX_E_INVALID, "negative token count");
   if (num_tokens == 0 || c.num_blocks == 0) return KVX_OK;
   if (!slot_mapping) return set_error(KVX_E_INVALID, "slot_mapping is NULL");
-  if (num_tokens > kMostGrid) return set_error(KVX_E_UNSUPPORTED, "too many tokens for one launch");
+  if (num_tokens > INT32_MAX - 2048 || slices_grid(num_tokens <= 1024 ? num_tokens : num_tokens / 16 + 1, 2 * c.heads) > kMostGrid)
+    return set_error(KVX_E_UNSUPPORTED, "too many tokens for one launch");
   const int64_t row = (int64_t)c.heads * c.head_dim;
   if ((rc = check_rows("key", key, key_stride, num_tokens, row, dtype))) return rc;
   if ((rc = check_rows("value", value, value_stride, num_tokens, row, dtype))) return rc;
@@ -220,7 +221,7 @@ int kvx_attention_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, 
     return set_error(KVX_E_INVALID, "attention needs %lld bytes of workspace on 16 bytes (got %lld)", (long long)need,
                      (long long)workspace_bytes);
   a.partial = (float*)workspace;
-  if ((int64_t)a.batch.num_seqs * a.cache.heads * a.splits * a.row_tiles > kMostGrid / 2 ||
+  if (slices_grid((int64_t)a.batch.num_seqs * a.splits * a.row_tiles, a.cache.heads) > kMostGrid / 2 ||
       (int64_t)a.batch.max_seqlen * query_heads > kMostGrid)
     return set_error(KVX_E_UNSUPPORTED, "too many sequences, heads and queries for one launch");
   return hip_status(launch_attention(a, dtype, (hipStream_t)stream), "attention_fp8 launch");
@@ -238,7 +239,7 @@ int kvx_attention_weights_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch*
   if (a.batch.num_seqs == 0 || width == 0) return KVX_OK;
   if (!out || (a.batch.num_tokens > 0 && !lse)) return set_error(KVX_E_INVALID, "NULL tensor pointer");
   if (!spans(a.batch.num_seqs, a.cache.heads, width, 4) ||
-      (int64_t)a.batch.num_seqs * a.cache.heads * (width / 128 + 1) > kMostGrid)
+      slices_grid((int64_t)a.batch.num_seqs * (width / 128 + 1), a.cache.heads) > kMostGrid)
     return set_error(KVX_E_UNSUPPORTED, "too many weights for one launch");
   a.query = query;
   a.q_stride = query_stride;
@@ -282,7 +283,8 @@ int kvx_compact_kvcache_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* f
   if (!indices || !counts || !to_tables) return set_error(KVX_E_INVALID, "NULL tensor pointer");
   if ((int64_t)to_width * c.block_size < keep)
     return set_error(KVX_E_RANGE, "%d blocks of %d tokens do not hold %d", to_width, c.block_size, keep);
-  if (keep > INT32_MAX - 2048 || !spans(b.num_seqs, c.heads, keep, 4))
+  if (keep > INT32_MAX - 2048 || !spans(b.num_seqs, c.heads, keep, 4) ||
+      slices_grid(((int64_t)keep / c.group + 1) * b.num_seqs, 2 * c.heads) > kMostGrid)
     return set_error(KVX_E_UNSUPPORTED, "too many tokens for one launch");
   return hip_status(launch_compact(c, b, indices, counts, keep, to_tables, to_stride, to_width, (hipStream_t)stream),
                     "compact_kvcache_fp8 launch");

@@ -186,10 +186,12 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
   __shared__ int wave_end[kThreads / kWave];
   __shared__ float wave_amax[kThreads / kWave];
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int head = blockIdx.y % c.heads;
-  const bool is_v = blockIdx.y >= c.heads;
+  const Slice slice = slice_of(blockIdx.x, 2 * c.heads);
+  const bool is_v = slice.head >= c.heads;
+  const int head = is_v ? slice.head - c.heads : slice.head;
   const int64_t cache_slots = (int64_t)c.num_blocks * c.block_size;
-  const int first = blockIdx.x * chunk;
+  const int first = slice.unit * chunk;
+  if (first >= num_tokens) return;
   auto group_at = [&](int token) {  // -1 where the token is skipped or none
     if (token < 0 || token >= num_tokens) return -1;
     const int s = slots[token];
@@ -481,11 +483,14 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   __shared__ float wave_amax[kThreads / kWave];
   __shared__ int64_t source[kMaxGroup];  // slot of each row, or -1
   __shared__ float source_scale[kMaxGroup];
-  const int tid = threadIdx.x, head = blockIdx.y % c.heads, seq = blockIdx.z;
-  const bool is_v = blockIdx.y >= c.heads;
+  const int tid = threadIdx.x;
+  const Slice slice = slice_of(blockIdx.x, 2 * c.heads);
+  const int seq = slice.unit % from.num_seqs;
+  const bool is_v = slice.head >= c.heads;
+  const int head = is_v ? slice.head - c.heads : slice.head;
   int count = counts[seq];
   count = count < 0 ? 0 : count > keep ? keep : count;
-  const int first = blockIdx.x * c.group;
+  const int first = slice.unit / from.num_seqs * c.group;
   if (first >= count) return;
   const int rows = count - first < c.group ? count - first : c.group;
   const int to_block = c.block_of(first);
@@ -588,7 +593,8 @@ hipError_t store_of(const Fp8Cache& c, const void* key, int64_t key_stride, cons
   int lane_bits = 1;
   while ((8 << lane_bits) < c.head_dim) ++lane_bits;
   const int chunk = num_tokens <= kStoreSingle ? 1 : 16;
-  store_fp8_kernel<T><<<dim3((unsigned)((num_tokens + chunk - 1) / chunk), (unsigned)(2 * c.heads)), dim3(kThreads), 0, stream>>>(
+  const dim3 grid((unsigned)slices_grid((num_tokens + chunk - 1) / chunk, 2 * c.heads));
+  store_fp8_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(
       c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens, chunk, lane_bits);
   return hipGetLastError();
 }
@@ -624,7 +630,7 @@ hipError_t launch_select(const float* weights, int32_t rows, int32_t heads, int3
 hipError_t launch_compact(const Fp8Cache& c, const PagedBatch& from, const int32_t* indices, const int32_t* counts,
                           int32_t keep, const int32_t* to_tables, int64_t to_stride, int32_t to_width,
                           hipStream_t stream) {
-  const dim3 grid((unsigned)((keep + c.group - 1) / c.group), (unsigned)(2 * c.heads), (unsigned)from.num_seqs);
+  const dim3 grid((unsigned)slices_grid((int64_t)((keep + c.group - 1) / c.group) * from.num_seqs, 2 * c.heads));
   int lane_bits = 0;
   while ((16 << lane_bits) < c.head_dim) ++lane_bits;
   compact_kernel<<<grid, dim3(kThreads), 0, stream>>>(c, from, indices, counts, keep, to_tables, to_stride, to_width,
