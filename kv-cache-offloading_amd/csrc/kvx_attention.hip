@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
   const int seq = slice.unit % a.batch.num_seqs, rest = slice.unit / a.batch.num_seqs, head = slice.head;
   const int tile = rest % a.row_tiles, split = rest / a.row_tiles;
   if (split >= a.splits) return;
-  const int context = cache.num_blocks > 0 ? context_of(a.batch, seq, cache.block_size) : 0;
+  const int context = context_of(cache, a.batch, seq);
   const int first_step = split * a.split_steps;
   // The first split also writes the rows that see nothing.
   if (first_step * kStep >= context && split > 0) return;
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
     u32x4 k_codes[2][kChunks];
     uint32_t v_codes[8][kCols / 4];
     int64_t info_row = -1;  // of tile lane % 2 of the batch's step lane / 2
-    float info_k = 0.0f, info_v = 0.0f;
+    float info_k = 0.0f, info_v = 0.0f;  // as loaded: used at once, they would hold up the codes' loads
     auto look_up = [&](int nth) {
       const int step = my_first + (nth + lane / 2) * kWaves, key = step * kStep + lane % 2 * 16;
       info_row = -1;
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         if (id >= 0 && id < cache.num_blocks) {
           info_row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
           const int64_t at = ((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head;
-          info_k = cache.k_scale[at] * a.scale;
+          info_k = cache.k_scale[at];
           info_v = cache.v_scale[at];
         }
       }
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
       for (int t = 0; t < 2; ++t) {
         const int at = nth % 32 * 2 + t;
         there[t] = row_of(nth, t) >= 0;
-        ks[t] = lane_value(info_k, at);
+        ks[t] = lane_value(info_k, at) * a.scale;
         vs[t] = lane_value(info_v, at);
       }
       f32x4 s[kTiles][2];
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
   const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
   const int tile = a.row_tiles - 1 - rest % a.row_tiles, split = rest / a.row_tiles;  // the longest first
   const int seq = pair / cache.heads, head = pair % cache.heads;
-  const int context = context_of(a.batch, seq, cache.block_size);
+  const int context = context_of(cache, a.batch, seq);
   const int split_passes = a.split_steps * kStep / kKeys, first_pass = split * split_passes;
   if (first_pass * kKeys >= context && split > 0) return;  // the first split also writes the rows that see nothing
   const QueryRows rows = query_rows(a.batch, seq);
@@ -895,52 +895,66 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
   }
 }
 
-// Joins the splits: a workgroup per query row, its threads over 4 columns of one split after another.
+// Joins the splits: a workgroup per query row, its threads over 4 columns of one split after another. All parts are
+// asked for at once, with the sums that weigh them: waited for by turns, 128 splits took 10 us.
 constexpr int kMaxSplits = 128;
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttentionArgs a) {
+template <typename T, int kJoinThreads>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttentionArgs a) {
+  constexpr int kHeld = 4, kJoinWaves = kJoinThreads / kWave;
   __shared__ float fades[kMaxSplits];
-  __shared__ float wave_top[kWaves], wave_sum[kWaves];
-  __shared__ f32x4 parts[kThreads];
+  __shared__ float wave_top[kJoinWaves], wave_sum[kJoinWaves];
+  __shared__ f32x4 parts[kJoinThreads];
   const int tid = threadIdx.x, seq = blockIdx.y, hd = a.cache.head_dim;
   const QueryRows rows = query_rows(a.batch, seq);
-  const int context = context_of(a.batch, seq, a.cache.block_size);
+  const int context = context_of(a.cache, a.batch, seq);
   const int steps = (context + kStep - 1) / kStep, used = steps <= a.split_steps ? 1 : (steps - 1) / a.split_steps + 1;
   const int64_t total_rows = (int64_t)a.batch.num_tokens * a.q_heads;
   const float* stats = a.partial + a.splits * total_rows * hd;
-  const int columns = hd <= 64 ? 16 : hd <= 128 ? 32 : 64, groups = kThreads / columns;  // threads of 4 columns
-  const int col = tid % columns * 4, group = tid / columns;
+  const int columns = hd <= 64 ? 16 : hd <= 128 ? 32 : 64, groups = kJoinThreads / columns;  // threads of 4 columns
+  const int col = min(tid % columns * 4, hd - 4), group = tid / columns;
   for (int r = blockIdx.x; r < rows.count * a.q_heads; r += gridDim.x) {
     const int64_t row = (int64_t)rows.first * a.q_heads + r;
-    f32x2 mine = {-INFINITY, 0.0f};
-    if (tid < used) mine = *reinterpret_cast<const f32x2*>(stats + (tid * total_rows + row) * 2);
-    float top = mine.x;
+    const float* from = a.partial + row * hd + col;
+    const f32x2 mine = *reinterpret_cast<const f32x2*>(stats + ((tid < used ? tid : 0) * total_rows + row) * 2);
+    f32x4 part[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int s = group + i * groups;
+      part[i] = *reinterpret_cast<const f32x4*>(from + (s < used ? s : 0) * total_rows * hd);
+    }
+    const float my_sum = tid < used ? mine.y : 0.0f;
+    float top = tid < used ? mine.x : -INFINITY;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     if (tid % kWave == 0) wave_top[tid / kWave] = top;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_top[w]);
-    const float fade = mine.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mine.x - top);
-    float sum = mine.y == 0.0f ? 0.0f : mine.y * fade;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, wave_top[w]);
+    const float fade = my_sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mine.x - top);
+    float sum = my_sum == 0.0f ? 0.0f : my_sum * fade;
     if (tid < used) fades[tid] = fade;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
     if (tid % kWave == 0) wave_sum[tid / kWave] = sum;
     __syncthreads();
     sum = 0.0f;
-    for (int w = 0; w < kWaves; ++w) sum += wave_sum[w];
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) sum += wave_sum[w];
     f32x4 y = {0, 0, 0, 0};
-    if (col < hd) {
-#pragma unroll 4
-      for (int s = group; s < used; s += groups) {
-        const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial + (s * total_rows + row) * hd + col);
-        if (fades[s] != 0.0f) y += part * fades[s];
-      }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int s = group + i * groups;
+      const float times = s < used ? fades[s] : 0.0f;
+      if (times != 0.0f) y += part[i] * times;  // a part of sum 0 may hold anything
+    }
+    for (int s = group + kHeld * groups; s < used; s += groups) {
+      const f32x4 more = *reinterpret_cast<const f32x4*>(from + s * total_rows * hd);
+      if (fades[s] != 0.0f) y += more * fades[s];
     }
     parts[tid] = y;
     __syncthreads();
-    if (group == 0 && col < hd) {
-      for (int i = 1; i < groups; ++i) y += parts[i * columns + tid];
+    if (group == 0 && tid % columns * 4 < hd) {
+      for (int i = 1; i < groups && i < used; ++i) y += parts[i * columns + tid];
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       alignas(8) T out[4];
 #pragma unroll
@@ -973,15 +987,16 @@ __device__ __forceinline__ WeightRow<T> weight_row(const WeightsArgs& a, const Q
   WeightRow<T> row;
   row.query = (const T*)a.query + (int64_t)(rows.first + nth) * a.q_stride + (int64_t)q_head * a.cache.head_dim;
   row.last = real ? context - rows.count + nth : -1;
-  const float lse = real ? a.lse[(int64_t)(rows.first + nth) * a.q_heads + q_head] : -INFINITY;
-  row.lse = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+  row.lse = a.lse[real ? (int64_t)(rows.first + nth) * a.q_heads + q_head : 0];
+  if (!real) row.lse = -INFINITY;
+  row.lse = row.lse == -INFINITY ? INFINITY : row.lse * 1.4426950408889634f;
   return row;
 }
 
 // 16 adjacent keys' lookup, a lane for each.
 struct KeyTile {
   int64_t row;  // slot * heads + head of the first key, or -1
-  float scale;
+  float scale;  // as loaded: multiplied at once, it would hold up K's loads
 };
 __device__ __forceinline__ KeyTile key_tile(const WeightsArgs& a, const int32_t* table, int context, int head, int key) {
   const Fp8Cache& cache = a.cache;
@@ -991,8 +1006,7 @@ __device__ __forceinline__ KeyTile key_tile(const WeightsArgs& a, const int32_t*
     const int id = table[block];
     if (id >= 0 && id < cache.num_blocks) {
       t.row = ((int64_t)id * cache.block_size + in) * cache.heads + head;
-      t.scale = cache.k_scale[((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head] *
-                a.scale;
+      t.scale = cache.k_scale[((int64_t)id * (cache.block_size / cache.group) + cache.group_of(in)) * cache.heads + head];
     }
   }
   return t;
@@ -1006,7 +1020,15 @@ __device__ __forceinline__ float sum16(float x) {
 }
 
 // Few query rows: bound by the bytes of K. A wave asks for kTiles * 16 keys at
-// once; its query rows come straight from memory, 16 at a time.
+// once; its query rows come straight from memory, 16 at a time. (Several turns
+// of so many keys, each turn's asked for during the one before, took 32 us in
+// place of 27 for 16 contexts of 2-8 K tokens, whose waves are few, and 142 in
+// place of 144 for 64 of 32 K tokens on 2 heads.)
+__device__ __forceinline__ void copy_weights(const WeightsArgs& a, int64_t at, int count, int lane) {  // nothing is added
+  if (a.weights == a.out) return;
+  for (int i = lane; i < count; i += kWave) a.out[at + i] = a.weights ? a.weights[at + i] : 0.0f;
+}
+
 template <int kType, int kHd, int kTiles>
 __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
   using Q = Query<kType>;
@@ -1020,17 +1042,12 @@ __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
   const int seq = slice.unit % a.batch.num_seqs, head = slice.head, pair = seq * cache.heads + head;
   const int key0 = (slice.unit / a.batch.num_seqs * kWaves + wave) * kTiles * 16;
   if (key0 >= a.width) return;
-  const int context = context_of(a.batch, seq, cache.block_size);
+  const int context = context_of(cache, a.batch, seq);
   const int64_t base = (int64_t)pair * a.width;
-  if (key0 >= context) {  // nothing is added
-    if (a.weights != a.out) {
-      for (int key = key0 + lane; key < key0 + kTiles * 16 && key < a.width; key += kWave)
-        a.out[base + key] = a.weights ? a.weights[base + key] : 0.0f;
-    }
-    return;
-  }
+  if (key0 >= context) return copy_weights(a, base + key0, min(kTiles * 16, a.width - key0), lane);
   const QueryRows rows = query_rows(a.batch, seq);
   const int num_rows = rows.count * a.per_kv;
+  if (num_rows == 0) return copy_weights(a, base + key0, min(kTiles * 16, a.width - key0), lane);
   WeightRow<T> row = weight_row<T>(a, rows, context, head, c);
   const KeyTile mine = key_tile(a, a.batch.tables + seq * a.batch.table_stride, lane < kTiles ? context : 0, head,
                                 key0 + lane * 16);
@@ -1040,7 +1057,7 @@ __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
     const int64_t at = lane_value(mine.row, t);
-    scale[t] = lane_value(mine.scale, t);
+    scale[t] = lane_value(mine.scale, t) * a.scale;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       k[t][i] = u32x4{0, 0, 0, 0};
@@ -1127,7 +1144,7 @@ __global__ __launch_bounds__(kThreads) void weights_many_kernel(WeightsArgs a) {
   const int pairs = a.batch.num_seqs * cache.heads;
   const int pair = blockIdx.x % pairs, seq = pair / cache.heads, head = pair % cache.heads;
   const int group0 = (blockIdx.x / pairs) * kWaves * 32, key0 = group0 + wave * 32;
-  const int context = context_of(a.batch, seq, cache.block_size);
+  const int context = context_of(cache, a.batch, seq);
   const int64_t base = (int64_t)pair * a.width;
   const QueryRows rows = query_rows(a.batch, seq);
   const int num_rows = group0 < context ? rows.count * a.per_kv : 0;
@@ -1135,7 +1152,7 @@ __global__ __launch_bounds__(kThreads) void weights_many_kernel(WeightsArgs a) {
   const KeyTile mine = key_tile(a, a.batch.tables + seq * a.batch.table_stride, lane < 2 ? context : 0, head,
                                 key0 + lane * 16);
   const bool there[2] = {lane_value(mine.row, 0) >= 0, lane_value(mine.row, 1) >= 0};
-  const float scale[2] = {lane_value(mine.scale, 0), lane_value(mine.scale, 1)};
+  const float scale[2] = {lane_value(mine.scale, 0) * a.scale, lane_value(mine.scale, 1) * a.scale};
   // K: lane (n, h) holds columns 16 d + 8 h .. of key n.
   Vec k[kDots];
   {
@@ -1278,7 +1295,8 @@ hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
   }
   if (err != hipSuccess || a.splits == 1) return err;
   const dim3 grid((unsigned)((int64_t)a.batch.max_seqlen * a.q_heads), (unsigned)a.batch.num_seqs);
-  join_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(a);
+  if (a.splits <= 16) join_kernel<T, 256><<<grid, dim3(256), 0, stream>>>(a);
+  else join_kernel<T, 1024><<<grid, dim3(1024), 0, stream>>>(a);
   return hipGetLastError();
 }
 

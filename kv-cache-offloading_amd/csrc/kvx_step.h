@@ -161,9 +161,9 @@ __device__ __forceinline__ Slice slice_of(unsigned bid, int heads) {
 }
 __host__ inline int64_t slices_grid(int64_t units, int64_t heads) { return (units + 7) / 8 * 8 * heads; }
 
-// Tokens of sequence b that are cached, as its table can hold them.
-__device__ __forceinline__ int context_of(const PagedBatch& b, int seq, int block_size) {
-  const int64_t room = (int64_t)b.table_width * block_size;
+// Tokens of sequence b that are cached, as its table can hold them; none in a cache without blocks.
+__device__ __forceinline__ int context_of(const Fp8Cache& c, const PagedBatch& b, int seq) {
+  const int64_t room = c.num_blocks > 0 ? (int64_t)b.table_width * c.block_size : 0;
   if (!b.context_lens) return (int)room;
   const int n = b.context_lens[seq];
   return n < 0 ? 0 : n > room ? (int)room : n;

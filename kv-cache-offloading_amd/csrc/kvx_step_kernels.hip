@@ -501,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   float* scales = is_v ? c.v_scale : c.k_scale;
   const int64_t to_slot = (int64_t)target * c.block_size + (first - to_block * c.block_size);
   const int32_t* mine = indices + ((int64_t)seq * c.heads + head) * keep + first;
-  const int context = context_of(from, seq, c.block_size);
+  const int context = context_of(c, from, seq);
   for (int i = tid; i < rows; i += kThreads) {
     const int t = mine[i];
     int64_t slot = -1;

@@ -217,6 +217,34 @@ def test_no_sequences_and_no_rows(gpu):
     assert torch.equal(same, weights)
 
 
+@pytest.mark.parametrize("q_lens", [[0, 3, 0], [40, 0, 0], [0, 0, 70]])
+def test_sequences_without_rows(gpu, q_lens):
+    s = Setup(gpu, [50, 90, 300], q_lens, 2, 2, 64, 16, 16)
+    s.check()
+    where, how = s.batch()
+    _, lse = s.run()
+    before = torch.rand((3, 2, s.tables.shape[1] * 16), device=gpu)
+    got = ops.attention_weights_fp8(s.q.to(gpu), lse, fp8(s.k, gpu), s.ks.to(gpu), *where, s.scale, weights=before,
+                                    out=torch.empty_like(before), **how)
+    for b, n in enumerate(q_lens):
+        assert n or torch.equal(got[b], before[b])
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_a_cache_without_blocks(gpu, rows):
+    q = query(rows, 4, 64, torch.bfloat16, 1).to(gpu)
+    codes = torch.empty((0, 256, 2, 64), dtype=torch.uint8, device=gpu).view(torch.float8_e4m3fn)
+    scales = torch.empty((0, 4, 2, 1), device=gpu)
+    tables, lens = torch.zeros((1, 40), dtype=torch.int32, device=gpu), int32([9000], gpu)
+    how = dict(cu_seqlens=int32([0, rows], gpu), max_seqlen=rows)
+    out, lse = ops.attention_fp8(q, codes, codes, scales, scales, tables, lens, return_lse=True, **how)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    weights = torch.rand((1, 2, 500), device=gpu)
+    got = ops.attention_weights_fp8(q, lse, codes, scales, tables, lens, weights=weights, out=torch.empty_like(weights), **how)
+    assert torch.equal(got, weights)
+    ops.store_kvcache_fp8(q[:, :2], q[:, 2:], codes, codes, scales, scales, int32([0] * rows, gpu))
+
+
 def test_large_scores_and_scales(gpu):
     s = Setup(gpu, [100, 50], None, 1, 4, 64, 32, 32)
     s.q *= 300.0  # scores of hundreds: one token takes nearly all
