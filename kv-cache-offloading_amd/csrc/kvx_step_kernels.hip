@@ -481,8 +481,7 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
                                                            int32_t to_width, int32_t lane_bits) {
   constexpr int kHold = 2;
   __shared__ float wave_amax[kThreads / kWave];
-  __shared__ int64_t source[kMaxGroup];  // slot of each row, or -1
-  __shared__ float source_scale[kMaxGroup];
+  __shared__ int64_t source[kMaxGroup], source_scale[kMaxGroup];  // each row's slot, or -1, and its scale's element
   const int tid = threadIdx.x;
   const Slice slice = slice_of(blockIdx.x, 2 * c.heads);
   const int seq = slice.unit % from.num_seqs;
@@ -504,14 +503,13 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   const int context = context_of(c, from, seq);
   for (int i = tid; i < rows; i += kThreads) {
     const int t = mine[i];
-    int64_t slot = -1;
-    float scale = 0.0f;
+    int64_t slot = -1, scale = 0;
     if (t >= 0 && t < context) {
       const int b = c.block_of(t), in = t - b * c.block_size;
       const int id = from.tables[seq * from.table_stride + b];
       if (id >= 0 && id < c.num_blocks) {
         slot = (int64_t)id * c.block_size + in;
-        scale = scales[((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head];
+        scale = ((int64_t)id * (c.block_size / c.group) + c.group_of(in)) * c.heads + head;
       }
     }
     source[i] = slot;
@@ -520,32 +518,39 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   __syncthreads();
   const int at = (tid & ((1 << lane_bits) - 1)) * 16, row0 = tid >> lane_bits, row_step = kThreads >> lane_bits;
   const bool in_row = at < c.head_dim;
+  // A row's piece and its scale.
+  struct Row {
+    u32x4 codes;
+    float scale;
+  };
   auto read = [&](int row) {
-    u32x4 w = {0, 0, 0, 0};
-    if (row < rows && in_row && source[row] >= 0)
-      w = *reinterpret_cast<const u32x4*>(codes + (source[row] * c.heads + head) * c.head_dim + at);
-    return w;
+    Row r = {u32x4{0, 0, 0, 0}, 0.0f};
+    if (row < rows && in_row && source[row] >= 0) {
+      r.codes = *reinterpret_cast<const u32x4*>(codes + (source[row] * c.heads + head) * c.head_dim + at);
+      r.scale = scales[source_scale[row]];
+    }
+    return r;
   };
-  auto value = [&](const u32x4& w, float scale, float* x) {
+  auto value = [&](const Row& r, float* x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) decode4(w[i], x + 4 * i);
+    for (int i = 0; i < 4; ++i) decode4(r.codes[i], x + 4 * i);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= scale;
+    for (int i = 0; i < 16; ++i) x[i] *= r.scale;
   };
-  auto amax_of = [&](const u32x4& w, int row) {
+  auto amax_of = [&](const Row& r) {
     float x[16], most = 0.0f;
-    value(w, row < rows ? source_scale[row] : 0.0f, x);
+    value(r, x);
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = fmaxf(most, finite_abs(x[i]));
     return most;
   };
-  u32x4 held[kHold];
+  Row held[kHold];
   float amax = 0.0f;
 #pragma unroll
   for (int p = 0; p < kHold; ++p) held[p] = read(row0 + p * row_step);
 #pragma unroll
-  for (int p = 0; p < kHold; ++p) amax = fmaxf(amax, amax_of(held[p], row0 + p * row_step));
-  for (int row = row0 + kHold * row_step; row < rows; row += row_step) amax = fmaxf(amax, amax_of(read(row), row));
+  for (int p = 0; p < kHold; ++p) amax = fmaxf(amax, amax_of(held[p]));
+  for (int row = row0 + kHold * row_step; row < rows; row += row_step) amax = fmaxf(amax, amax_of(read(row)));
   amax = wave_max(amax);
   if (tid % kWave == 0) wave_amax[tid / kWave] = amax;
   __syncthreads();
@@ -554,10 +559,10 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   const float fit = scale_for(amax), inverse = 1.0f / fit;
   if (tid == 0)
     scales[((int64_t)target * (c.block_size / c.group) + c.group_of(first - to_block * c.block_size)) * c.heads + head] = fit;
-  auto write = [&](const u32x4& w, int row) {
+  auto write = [&](const Row& r, int row) {
     if (row >= rows || !in_row) return;
     float x[16];
-    value(w, source_scale[row], x);
+    value(r, x);
     const u32x2 lo = encode8(x, inverse), hi = encode8(x + 8, inverse);
     *reinterpret_cast<u32x4*>(codes + ((to_slot + row) * c.heads + head) * c.head_dim + at) = u32x4{lo.x, lo.y, hi.x, hi.y};
   };
@@ -584,7 +589,8 @@ hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Up to so many tokens each is looked at by workgroups of its own, as a decode step's begin a group each.
+// Up to so many tokens each is looked at by workgroups of its own, as a decode step's begin a group each. More are taken
+// to be prompts, by as many as a group has, up to a wave: most workgroups then find one group that begins.
 constexpr int kStoreSingle = 1024;
 
 template <typename T>
@@ -592,7 +598,7 @@ hipError_t store_of(const Fp8Cache& c, const void* key, int64_t key_stride, cons
                     const int32_t* slots, int32_t num_tokens, hipStream_t stream) {
   int lane_bits = 1;
   while ((8 << lane_bits) < c.head_dim) ++lane_bits;
-  const int chunk = num_tokens <= kStoreSingle ? 1 : 16;
+  const int chunk = num_tokens <= kStoreSingle ? 1 : c.group < kWave ? c.group : kWave;
   const dim3 grid((unsigned)slices_grid((num_tokens + chunk - 1) / chunk, 2 * c.heads));
   store_fp8_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(
       c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens, chunk, lane_bits);
