@@ -243,8 +243,8 @@ int kvx_rotary_embed(const void* query, int64_t query_stride, const void* key, i
  * group's first slot, the group goes on: its scale is the larger of that and
  * the one it had, and if that grew, its other rows are encoded anew. Where it
  * does, the group starts over, and rows that the call does not write hold
- * nothing. The tokens of one group stand together in the call; of two with one
- * slot the later one is stored.
+ * nothing. The tokens of one group stand together in the call, with none of
+ * another group between them; of two with one slot the later one is stored.
  */
 int kvx_store_kvcache_fp8(const kvx_fp8_cache* cache, const void* key, int64_t key_stride, const void* value,
                           int64_t value_stride, int32_t dtype, const int32_t* slot_mapping, int64_t num_tokens,
@@ -254,6 +254,7 @@ int kvx_store_kvcache_fp8(const kvx_fp8_cache* cache, const void* key, int64_t k
  * Causal attention over an e4m3 cache: out[row, head] = softmax(softmax_scale *
  * q . K) V over the tokens that the row sees, lse the logarithm of the sum of
  * exp(scores) (NULL: not written); 0 and -infinity for a row that sees none.
+ * softmax_scale and the cache's scales are positive.
  * query_heads is a multiple of H; head h reads KV head h / (query_heads / H).
  * out: [num_tokens, query_heads, hd] of the query's type, lse: [num_tokens,
  * query_heads]. `workspace`: as many bytes as kvx_attention_fp8_workspace

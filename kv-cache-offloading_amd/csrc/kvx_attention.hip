@@ -1127,7 +1127,7 @@ __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
 // time, through LDS, and a wave computes the scores of the next 32 of them under
 // the exponentials of these.
 template <int kType, int kHd>
-__global__ __launch_bounds__(kThreads) void weights_many_kernel(WeightsArgs a) {
+__global__ __launch_bounds__(kThreads, kHd < 256 ? 3 : 2) void weights_many_kernel(WeightsArgs a) {
   using Q = Query<kType>;
   using T = typename Q::T;
   using Vec = typename Q::Vec;

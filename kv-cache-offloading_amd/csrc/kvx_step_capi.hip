@@ -98,13 +98,15 @@ int check_batch(const kvx_paged_batch* b, const Fp8Cache& c, PagedBatch* out, bo
 }
 
 int check_queries(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads, const void* query, int64_t q_stride,
-                  int32_t dtype) {
+                  int32_t dtype, float softmax_scale) {
   int rc = check_dtype(dtype, false);
   if (rc) return rc;
   if (q_heads <= 0 || q_heads % c.heads)
     return set_error(KVX_E_INVALID, "%d query heads are not a multiple of %d KV heads", q_heads, c.heads);
-  if ((int64_t)b.num_tokens * q_heads > (int64_t)INT32_MAX - 2048)
-    return set_error(KVX_E_UNSUPPORTED, "more than 2^31 query rows");
+  if (!(softmax_scale > 0.0f && softmax_scale < INFINITY))
+    return set_error(KVX_E_INVALID, "softmax_scale must be positive and finite");
+  if ((int64_t)b.num_tokens * q_heads > int64_t{1} << 30)
+    return set_error(KVX_E_UNSUPPORTED, "more than 2^30 query rows");
   return check_rows("query", query, q_stride, b.num_tokens, (int64_t)q_heads * c.head_dim, dtype);
 }
 
@@ -199,7 +201,7 @@ int kvx_attention_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, 
   AttentionArgs a{};
   int rc = check_cache(cache, true, &a.cache);
   if (!rc) rc = check_batch(batch, a.cache, &a.batch);
-  if (!rc) rc = check_queries(a.cache, a.batch, query_heads, query, query_stride, dtype);
+  if (!rc) rc = check_queries(a.cache, a.batch, query_heads, query, query_stride, dtype, softmax_scale);
   if (rc) return rc;
   if (a.batch.num_seqs == 0 || a.batch.num_tokens == 0) return KVX_OK;
   if (!out) return set_error(KVX_E_INVALID, "out is NULL");
@@ -233,7 +235,7 @@ int kvx_attention_weights_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch*
   WeightsArgs a{};
   int rc = check_cache(cache, false, &a.cache);
   if (!rc) rc = check_batch(batch, a.cache, &a.batch);
-  if (!rc) rc = check_queries(a.cache, a.batch, query_heads, query, query_stride, dtype);
+  if (!rc) rc = check_queries(a.cache, a.batch, query_heads, query, query_stride, dtype, softmax_scale);
   if (rc) return rc;
   if (width < 0 || width > (int64_t)INT32_MAX - 2048) return set_error(KVX_E_INVALID, "bad width of the weights");
   if (a.batch.num_seqs == 0 || width == 0) return KVX_OK;

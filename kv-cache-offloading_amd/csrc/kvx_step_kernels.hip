@@ -197,7 +197,10 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
     const int s = slots[token];
     return s < 0 || s >= cache_slots ? -1 : c.group_of(s);
   };
-  const int mine = lane < chunk ? group_at(first + lane) : -1, before = lane < chunk ? group_at(first + lane - 1) : -1;
+  // Skipped tokens do not interrupt a group's: a token begins one if the last before it that is stored is not of it.
+  const int mine = lane < chunk ? group_at(first + lane) : -1;
+  int before = lane < chunk ? group_at(first + lane - 1) : -1;
+  for (int token = first + lane - 2; mine >= 0 && before < 0 && token >= 0; --token) before = group_at(token);
   uint64_t begins = __ballot(mine >= 0 && mine != before);
 
   const T* src = (is_v ? value : key) + (int64_t)head * c.head_dim;
@@ -216,14 +219,14 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
       const int i = from + tid;
       const int s = i < num_tokens ? slots[i] : -1;
       const bool in_group = s >= slot_base && s - slot_base < c.group;
-      const uint64_t out = ~__ballot(in_group);
+      const uint64_t out = __ballot(i >= num_tokens || (!in_group && s >= 0 && s < cache_slots));
       if (lane == 0) wave_end[wave] = out ? wave * kWave + __ffsll((unsigned long long)out) - 1 : kThreads;
       __syncthreads();
       int end = kThreads;
 #pragma unroll
       for (int w = kThreads / kWave - 1; w >= 0; --w)
         if (wave_end[w] < (w + 1) * kWave) end = wave_end[w];
-      if (tid < end) atomicMax(&owner[s - slot_base], i);
+      if (tid < end && in_group) atomicMax(&owner[s - slot_base], i);
       __syncthreads();
       if (end < kThreads) break;
     }

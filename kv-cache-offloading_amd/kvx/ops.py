@@ -361,8 +361,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
         def pair_turning(times: float) -> float:
             return rotary_dim * log(original_length / (times * 2 * pi)) / (2 * log(base))
 
-        low, high = max(0, floor(pair_turning(fast))), min(rotary_dim // 2 - 1, ceil(pair_turning(slow)))
-        blend = ((index - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)  # 0: stays, 1: divided
+        low, high = floor(pair_turning(fast)), ceil(pair_turning(slow))
+        blend = ((index - low) / max(high - low, 1)).clamp(0.0, 1.0)  # 0: stays, 1: divided
         frequencies = frequencies * (1 - blend) + frequencies / factor * blend
         magnitude = 0.1 * log(factor) + 1.0
     return frequencies.to(device), magnitude
@@ -473,7 +473,7 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     stride may differ). k_cache/v_cache: contiguous float8_e4m3fn [blocks, block_size, num_heads, head_dim] layer
     views, k_scale/v_scale: contiguous float32 [blocks, groups, num_heads, 1]; a group is block_size / groups tokens, a
     multiple of 16. slot_mapping: int32 [N], -1 and slots outside the cache skip a token; the tokens of one group
-    stand together in it, as those of a sequence do.
+    stand together in it, as those of a sequence do, with none of another group between them.
 
     A group's scale becomes the least power of two s with |x| <= 448 s for what the call writes there (s >= 2^-100;
     infinities saturate, NaN stays NaN). A call that does not write a group's first slot continues it: the scale is
@@ -527,7 +527,7 @@ def attention_fp8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     (row i of n sees the tokens up to context - n + i) and max_seqlen, the most rows of one (a hint that sizes the
     launch; default N). Rows of no sequence are left as they are; rows that see no token become 0. out: contiguous
     [N, q_heads, head_dim] of the query's type; lse: float32 [N, q_heads], log of the sum of exp(scores), -inf for
-    rows that see no token. softmax_scale defaults to head_dim ** -0.5. Capturable in a HIP graph.
+    rows that see no token. softmax_scale, positive, defaults to head_dim ** -0.5. Capturable in a HIP graph.
     """
     done = _bind().attention(query, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, softmax_scale,
                              cu_seqlens, max_seqlen, out, return_lse)

@@ -138,8 +138,8 @@ def c_batch(**change):
     return _lib.PagedBatch(**{**fields, **change})
 
 
-def attend(cache, batch, query=4096, stride=256, heads=4, dtype=_lib.DTYPE_BF16, out=4096, workspace=None, size=0):
-    _lib.check(_lib.lib().kvx_attention_fp8(ctypes.byref(cache), ctypes.byref(batch), query, stride, heads, dtype, 1.0, out,
+def attend(cache, batch, query=4096, stride=256, heads=4, dtype=_lib.DTYPE_BF16, out=4096, workspace=None, size=0, scale=1.0):
+    _lib.check(_lib.lib().kvx_attention_fp8(ctypes.byref(cache), ctypes.byref(batch), query, stride, heads, dtype, scale, out,
                                             None, workspace, size, None))
 
 
@@ -161,7 +161,8 @@ def test_c_caches_refused(change, error, match):
     (dict(heads=3), ValueError, "multiple"), (dict(dtype=_lib.DTYPE_FP32), NotImplementedError, "bf16 or fp16"), (dict(dtype=9), ValueError, "type"),
     (dict(query=4100), ValueError, "16 bytes"), (dict(stride=260), ValueError, "16 bytes"), (dict(out=None), ValueError, "out"),
     (dict(out=4098), ValueError, "16 bytes"), (dict(query=None), ValueError, "NULL"),
-    (dict(batch=dict(table_width=4000)), ValueError, "workspace")])
+    (dict(scale=0.0), ValueError, "positive"), (dict(scale=-1.0), ValueError, "positive"), (dict(scale=math.inf), ValueError, "positive"),
+    (dict(scale=math.nan), ValueError, "positive"), (dict(batch=dict(table_width=4000)), ValueError, "workspace")])
 def test_c_attention_refused(change, error, match):
     change = dict(change)
     batch = c_batch(**change.pop("batch", {}))

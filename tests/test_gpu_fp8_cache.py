@@ -128,6 +128,19 @@ def test_a_few_proposed_tokens(gpu, rows):
     Setup(gpu, lens, [rows] * 4, 2, 4, 128, 64, 32).check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [4, 8, 9, 40])
+def test_few_and_many_rows_behind_long_contexts(gpu, rows, hd):
+    # 16, 32, 36 and 160 rows a KV head, over several splits of the keys; some splits lie past a context.
+    Setup(gpu, [3000, 2047, 10, 0], [rows, rows, min(rows, 10), 0], 1, 4, hd, 64, 32, unused=NAN).check()
+
+
+def test_chunks_under_scales_that_are_no_powers_of_two(gpu):
+    # V is rounded to bf16 once more there: half a step besides P's.
+    for hd in (64, 128):
+        Setup(gpu, [300, 50], [60, 50], 1, 2, hd, 64, 32, powers=False).check(p_step=2.0 ** -7)
+
+
 @pytest.mark.parametrize("most", [1, 16, 300])
 def test_max_seqlen_is_only_a_hint(gpu, most):
     s = Setup(gpu, [200, 300], [150, 33], 1, 4, 64, 32, 32)
@@ -336,7 +349,8 @@ def test_calls_on_two_streams_at_once(gpu):
 @pytest.mark.parametrize("lens,q_lens,heads,per_kv,hd,block,group,dtype", [
     (LENGTHS, None, 2, 4, 128, 64, 32, torch.bfloat16), (LENGTHS, None, 1, 20, 80, 16, 16, torch.float16),
     ([67, 190, 40, 55, 3, 0], [67, 70, 0, 1, 9, 2], 2, 3, 64, 32, 16, torch.bfloat16),
-    ([300, 77], [300, 5], 1, 2, 256, 256, 64, torch.bfloat16), ([520], [64], 1, 8, 128, 64, 64, torch.bfloat16)])
+    ([300, 77], [300, 5], 1, 2, 256, 256, 64, torch.bfloat16), ([520], [64], 1, 8, 128, 64, 64, torch.bfloat16),
+    ([200, 33], [100, 33], 2, 3, 112, 64, 16, torch.float16), ([700, 9], [8, 9], 1, 4, 128, 64, 32, torch.bfloat16)])
 def test_weights(gpu, lens, q_lens, heads, per_kv, hd, block, group, dtype):
     s = Setup(gpu, lens, q_lens, heads, per_kv, hd, block, group, dtype, unused=NAN)
     _, lse, bound = s.want()
@@ -393,7 +407,8 @@ def pool(blocks, block, group, heads, hd, seed=0):
 @pytest.mark.parametrize("heads,hd,block,group,dtype", [
     (2, 128, 64, 32, torch.bfloat16), (1, 64, 16, 16, torch.float16), (3, 80, 48, 16, torch.float32),
     (2, 256, 64, 64, torch.bfloat16), (1, 16, 32, 32, torch.bfloat16), (8, 128, 256, 256, torch.bfloat16),
-    (1, 128, 1024, 1024, torch.float16), (5, 192, 32, 16, torch.float32)])
+    (1, 128, 1024, 1024, torch.float16), (5, 192, 32, 16, torch.float32),
+    (1, 64, 512, 16, torch.bfloat16)])
 def test_prompts_are_stored(gpu, heads, hd, block, group, dtype):
     lens = [1, block, 2 * block + 5, group + 1, 3]
     tables, blocks = tables_for(lens, block, 3)
@@ -418,6 +433,14 @@ def test_slots_in_any_order_within_a_group_and_outside_the_cache(gpu):
     slots = [5, 3, 4, -1, 96, 2 ** 31 - 1, -2 ** 31, 40, 33, 47, 95, 80, 70, 64, 71]
     check_store(gpu, rows(15, 2, 64, torch.bfloat16, 1), rows(15, 2, 64, torch.bfloat16, 2), caches, slots)
     check_store(gpu, rows(3, 2, 64, torch.bfloat16, 1), rows(3, 2, 64, torch.bfloat16, 2), caches, [-1, -1, 96])
+
+
+@pytest.mark.parametrize("gap", [1, 15, 70, 300, 1100])
+def test_skipped_tokens_do_not_interrupt_a_group(gpu, gap):
+    caches = pool(3, 32, 16, 1, 64)
+    slots = [3, 4] + [-1] * gap + [5, 10 ** 6, 6, 16] + [-1] * gap + [17, 40, -1, 41]
+    n = len(slots)
+    check_store(gpu, rows(n, 1, 64, torch.bfloat16, 1), rows(n, 1, 64, torch.bfloat16, 2), caches, slots)
 
 
 def test_the_later_of_two_tokens_with_one_slot_is_stored(gpu):
