@@ -26,11 +26,12 @@ struct Elem<KVX_DTYPE_FP32> {
   using T = float;
 };
 
-template <typename T>
-struct alignas(16) Piece {  // 16 bytes
-  static constexpr int kCount = 16 / sizeof(T);
+template <typename T, int kCount>
+struct alignas(sizeof(T) * kCount) Piece {  // read and written at once; 16 bytes at most
   T x[kCount];
 };
+template <typename T, int kVec>
+constexpr int kPieceOf = kVec * sizeof(T) > 16 ? 16 / sizeof(T) : kVec;
 
 // ---------------------------------------------------------------------------
 // Rotary positions: (a, b) -> (a cos - b sin, b cos + a sin) * magnitude with
@@ -44,33 +45,23 @@ struct alignas(16) Piece {  // 16 bytes
 
 template <typename T, int kVec>
 __device__ __forceinline__ void load_vec(const T* p, float* out) {
-  if constexpr (kVec * sizeof(T) >= 16) {
-    constexpr int kPer = Piece<T>::kCount;
+  constexpr int kPer = kPieceOf<T, kVec>;
 #pragma unroll
-    for (int i = 0; i < kVec / kPer; ++i) {
-      const Piece<T> piece = reinterpret_cast<const Piece<T>*>(p)[i];
+  for (int i = 0; i < kVec / kPer; ++i) {
+    const Piece<T, kPer> piece = reinterpret_cast<const Piece<T, kPer>*>(p)[i];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) out[i * kPer + j] = (float)piece.x[j];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) out[i] = (float)p[i];
+    for (int j = 0; j < kPer; ++j) out[i * kPer + j] = (float)piece.x[j];
   }
 }
 template <typename T, int kVec>
 __device__ __forceinline__ void store_vec(T* p, const float* in) {
-  if constexpr (kVec * sizeof(T) >= 16) {
-    constexpr int kPer = Piece<T>::kCount;
+  constexpr int kPer = kPieceOf<T, kVec>;
 #pragma unroll
-    for (int i = 0; i < kVec / kPer; ++i) {
-      Piece<T> piece;
+  for (int i = 0; i < kVec / kPer; ++i) {
+    Piece<T, kPer> piece;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) piece.x[j] = (T)in[i * kPer + j];
-      reinterpret_cast<Piece<T>*>(p)[i] = piece;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) p[i] = (T)in[i];
+    for (int j = 0; j < kPer; ++j) piece.x[j] = (T)in[i * kPer + j];
+    reinterpret_cast<Piece<T, kPer>*>(p)[i] = piece;
   }
 }
 
@@ -102,7 +93,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
            (int64_t)h * a.head_dim;
     float u[2 * kVec], w[2 * kVec];
     if (kInterleaved) {
-      load_vec<T, 2 * kVec>(x + 2 * at, u);
+      load_vec<T, kVec>(x + 2 * at, u);
+      load_vec<T, kVec>(x + 2 * at + kVec, u + kVec);
     } else {
       load_vec<T, kVec>(x + at, u);
       load_vec<T, kVec>(x + at + pairs, u + kVec);
@@ -115,7 +107,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
       w[second] = u[second] * t.x + u[first] * t.y;
     }
     if (kInterleaved) {
-      store_vec<T, 2 * kVec>(y + 2 * at, w);
+      store_vec<T, kVec>(y + 2 * at, w);
+      store_vec<T, kVec>(y + 2 * at + kVec, w + kVec);
     } else {
       store_vec<T, kVec>(y + at, w);
       store_vec<T, kVec>(y + at + pairs, w + kVec);
@@ -136,14 +129,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     T* y = is_key ? (T*)a.key_out + token * a.k_out_stride : (T*)a.query_out + token * a.q_out_stride;
     x += h * a.head_dim + at;
     y += h * a.head_dim + at;
-    if constexpr (kVec * sizeof(T) >= 16) {
-#pragma unroll
-      for (int j = 0; j < (int)(kVec * sizeof(T) / 16); ++j)
-        reinterpret_cast<u32x4*>(y)[j] = reinterpret_cast<const u32x4*>(x)[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = x[j];
-    }
+    *reinterpret_cast<Piece<T, kVec>*>(y) = *reinterpret_cast<const Piece<T, kVec>*>(x);
   }
 }
 
@@ -574,22 +560,31 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   for (int row = row0 + kHold * row_step; row < rows; row += row_step) write(read(row), row);
 }
 
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-
-template <typename T>
-hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
-  constexpr int kPer = 16 / sizeof(T);  // elements of a 16-byte piece
-  const int64_t strides[] = {a.q_stride, a.k_stride, a.q_out_stride, a.k_out_stride};
-  bool wide = aligned16(a.query) && aligned16(a.query_out) && aligned16(a.key) && aligned16(a.key_out) &&
-              a.head_dim % kPer == 0 && a.rotary_dim % (2 * kPer) == 0;
-  for (int64_t s : strides) wide = wide && s % kPer == 0;
+template <typename T, int kVec>
+hipError_t rotary_by(const RotaryArgs& a, hipStream_t stream) {
   const size_t lds = (size_t)a.rotary_dim / 2 * sizeof(float2);
   const dim3 grid((unsigned)a.num_tokens), block(kThreads);
-  if (wide && a.interleaved) rotary_kernel<T, kPer, true><<<grid, block, lds, stream>>>(a);
-  else if (wide) rotary_kernel<T, kPer, false><<<grid, block, lds, stream>>>(a);
-  else if (a.interleaved) rotary_kernel<T, 1, true><<<grid, block, lds, stream>>>(a);
-  else rotary_kernel<T, 1, false><<<grid, block, lds, stream>>>(a);
+  if (a.interleaved) rotary_kernel<T, kVec, true><<<grid, block, lds, stream>>>(a);
+  else rotary_kernel<T, kVec, false><<<grid, block, lds, stream>>>(a);
   return hipGetLastError();
+}
+
+// By 16 bytes where everything lies on 16 bytes, halves of the rotated part among it; by two elements likewise (a head_dim
+// of 80 with 20 rotated); else one by one.
+template <typename T>
+hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
+  auto lies_on = [&](int count) {
+    const int64_t elements[] = {a.q_stride, a.k_stride, a.q_out_stride, a.k_out_stride, a.head_dim, a.rotary_dim / 2};
+    const void* pointers[] = {a.query, a.key, a.query_out, a.key_out};
+    bool fits = true;
+    for (int64_t e : elements) fits = fits && e % count == 0;
+    for (const void* p : pointers) fits = fits && (uintptr_t)p % (count * sizeof(T)) == 0;
+    return fits;
+  };
+  constexpr int kWide = 16 / sizeof(T);
+  if (lies_on(kWide)) return rotary_by<T, kWide>(a, stream);
+  if (lies_on(2)) return rotary_by<T, 2>(a, stream);
+  return rotary_by<T, 1>(a, stream);
 }
 
 // Up to so many tokens each is looked at by workgroups of its own, as a decode step's begin a group each. More are taken

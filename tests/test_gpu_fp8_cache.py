@@ -502,7 +502,7 @@ def test_a_captured_store_replays(gpu):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("n,q_heads,k_heads,hd,rotary", [
-    (5, 4, 1, 128, 128), (1, 3, 2, 64, 32), (33, 2, 2, 80, 20), (7, 1, 0, 96, 96), (3, 0, 5, 256, 64), (4, 2, 1, 50, 2),
+    (5, 4, 1, 128, 128), (1, 3, 2, 64, 32), (33, 2, 2, 80, 20), (7, 1, 0, 96, 96), (3, 2, 1, 33, 12), (3, 0, 5, 256, 64), (4, 2, 1, 50, 2),
     (2, 8, 8, 192, 192), (700, 1, 1, 16, 16)])
 def test_rotary(gpu, n, q_heads, k_heads, hd, rotary, interleaved, dtype):
     g = torch.Generator().manual_seed(n)
@@ -532,7 +532,7 @@ def test_rotary(gpu, n, q_heads, k_heads, hd, rotary, interleaved, dtype):
             assert torch.equal(y[..., rotary:], x[..., rotary:])
 
 
-@pytest.mark.parametrize("hd,rotary", [(128, 64), (50, 20)])
+@pytest.mark.parametrize("hd,rotary", [(128, 64), (50, 20), (35, 10)])
 def test_rotary_in_place_and_into_views(gpu, hd, rotary):
     x = torch.randn((9, 6, hd), device=gpu).to(torch.bfloat16)
     positions, (frequencies, _) = torch.arange(9, device=gpu), ops.rotary_frequencies(rotary)
