@@ -145,6 +145,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // Which tokens begin a group is known on the device only. A workgroup looks at
 // `chunk` tokens and takes the groups that begin among them one after another.
 
+constexpr int kStoreHold = 4;
+
 template <typename T>
 struct Eight {  // elements, as loaded
   u32x4 w[sizeof(T) / 2];
@@ -162,12 +164,12 @@ __device__ __forceinline__ u32x2 encode8(const float* x, float times) {
   return out;
 }
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T* __restrict__ key, int64_t key_stride,
                                                              const T* __restrict__ value, int64_t value_stride,
                                                              const int32_t* __restrict__ slots, int32_t num_tokens,
                                                              int32_t chunk, int32_t lane_bits) {
-  constexpr int kHold = 4;
+  constexpr int kHold = kStoreHold;
   __shared__ int owner[kMaxGroup];  // the call's token for each of the group's rows; the last one that names it
   __shared__ int wave_end[kThreads / kWave];
   __shared__ float wave_amax[kThreads / kWave];
@@ -600,20 +602,35 @@ hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
   return rotary_by<T, 1>(a, stream);
 }
 
-// Up to so many tokens each is looked at by workgroups of its own, as a decode step's begin a group each. More are taken
-// to be prompts, by as many as a group has, up to a wave: most workgroups then find one group that begins.
-constexpr int kStoreSingle = 1024;
+// Workgroups are one wave where its lanes can hold a group (16 tokens of 128 elements: 16,384 tokens of 8 heads stored in 27
+// us, by four waves in 52), else four waves.
+// Each looks at as many tokens as leave so many workgroups, and at most at a group's, so that most of a prompt's find one
+// group that begins. A decode step's tokens begin a group each, which then wait for one another: with 2,048 / 4,096 / 8,192
+// workgroups of one wave 1,024 appended tokens of 8 heads take 20.7 / 13.9 / 14.4 us, as many of a prompt 6.6 / 8.6 / 14.3;
+// with 2,048 / 4,096 of four waves, in groups of 64, 41 / 41 and (4,096 tokens of a prompt) 15 / 26.
+constexpr int kStoreFull = 4096, kStoreFullWide = 2048;
 
+template <typename T, int kThreads>
+hipError_t store_by(const Fp8Cache& c, const void* key, int64_t key_stride, const void* value, int64_t value_stride,
+                    const int32_t* slots, int32_t num_tokens, int lane_bits, hipStream_t stream) {
+  const int most = c.group < kWave ? c.group : kWave;
+  int chunk = 1;
+  constexpr int kFull = kThreads == kWave ? kStoreFull : kStoreFullWide;
+  while (chunk < most && (int64_t)num_tokens * 2 * c.heads > (int64_t)chunk * kFull) chunk *= 2;
+  if (chunk > most) chunk = most;
+  const dim3 grid((unsigned)slices_grid((num_tokens + chunk - 1) / chunk, 2 * c.heads));
+  store_fp8_kernel<T, kThreads><<<grid, dim3(kThreads), 0, stream>>>(
+      c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens, chunk, lane_bits);
+  return hipGetLastError();
+}
 template <typename T>
 hipError_t store_of(const Fp8Cache& c, const void* key, int64_t key_stride, const void* value, int64_t value_stride,
                     const int32_t* slots, int32_t num_tokens, hipStream_t stream) {
   int lane_bits = 1;
   while ((8 << lane_bits) < c.head_dim) ++lane_bits;
-  const int chunk = num_tokens <= kStoreSingle ? 1 : c.group < kWave ? c.group : kWave;
-  const dim3 grid((unsigned)slices_grid((num_tokens + chunk - 1) / chunk, 2 * c.heads));
-  store_fp8_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(
-      c, (const T*)key, key_stride, (const T*)value, value_stride, slots, num_tokens, chunk, lane_bits);
-  return hipGetLastError();
+  if (c.group << lane_bits <= kStoreHold * kWave)
+    return store_by<T, kWave>(c, key, key_stride, value, value_stride, slots, num_tokens, lane_bits, stream);
+  return store_by<T, kThreads>(c, key, key_stride, value, value_stride, slots, num_tokens, lane_bits, stream);
 }
 
 }  // namespace
