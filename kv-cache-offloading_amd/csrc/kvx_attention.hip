@@ -1348,13 +1348,15 @@ AttentionPlan attention_plan(const Fp8Cache& c, const PagedBatch& b, int32_t q_h
   plan.row_tiles = (int32_t)((rows + tile_rows - 1) / tile_rows);
   const int64_t groups = (int64_t)b.num_seqs * c.heads * plan.row_tiles;
   const int64_t steps = ((int64_t)b.table_width * c.block_size + kStep - 1) / kStep;
-  // Split the keys while there are too few workgroups to fill the chip, each keeping 256 keys (chunks: 1,024) or more.
+  // Split the keys while there are too few workgroups to fill the chip, each keeping 256 keys or more (1,024: 16 chunks of
+  // 6 tokens and 8 query heads over 4 K 34.6 us, now 19.2). Chunks: up to one workgroup a CU, which is what one has LDS
+  // for (up to two, 256 of a chunk of 2,048 tokens over 8 K took 393 us, now 278; 160 of shorter ones 152 and 78).
   // Few rows: with few (sequence, KV head) pairs, one workgroup a CU, as the join takes its time for each split (8 pairs of
   // 32 K tokens in 128 / 64 / 32 / 16 splits 23.7 / 21.6 / 19.8 / 25.7 us); with more, some for each CU (64 pairs of 8 K in
   // 32 / 16 33.5 / 30.4); with many, so many that contexts of unlike lengths even out (61 of 300 to 8,192 tokens on 8 heads
   // in 4 / 8 splits 114 / 105; 2,048 pairs of 2 K in 2 / 1 219 / 203).
-  const int64_t want = !few ? 512 : groups < 16 ? 256 : groups < 256 ? 1024 : groups < 2048 ? 4096 : groups;
-  const int64_t unit = few ? 8 : chunk_keys(padded_head(c.head_dim)) / kStep, least = few ? 8 : 32;
+  const int64_t want = !few || groups < 16 ? 256 : groups < 256 ? 1024 : groups < 2048 ? 4096 : groups;
+  const int64_t unit = few ? 8 : chunk_keys(padded_head(c.head_dim)) / kStep, least = 8;
   int64_t splits = want / groups;
   if (splits > steps / least) splits = steps / least;
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
