@@ -602,12 +602,12 @@ hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
   return rotary_by<T, 1>(a, stream);
 }
 
-// Workgroups are one wave where its lanes can hold a group (16 tokens of 128 elements: 16,384 tokens of 8 heads stored in 27
-// us, by four waves in 52), else four waves.
+// Workgroups have one or two waves where their lanes can hold a group, else four: 16,384 tokens of 8 heads of 128 in groups
+// of 16 take 27 us by one wave and 52 by four, in groups of 32 28.5 by two and 34.5 by four.
 // Each looks at as many tokens as leave so many workgroups, and at most at a group's, so that most of a prompt's find one
 // group that begins. A decode step's tokens begin a group each, which then wait for one another: with 2,048 / 4,096 / 8,192
 // workgroups of one wave 1,024 appended tokens of 8 heads take 20.7 / 13.9 / 14.4 us, as many of a prompt 6.6 / 8.6 / 14.3;
-// with 2,048 / 4,096 of four waves, in groups of 64, 41 / 41 and (4,096 tokens of a prompt) 15 / 26.
+// with 2,048 / 4,096 of more waves, in groups of 64, 41 / 41 and (4,096 tokens of a prompt) 15 / 26.
 constexpr int kStoreFull = 4096, kStoreFullWide = 2048;
 
 template <typename T, int kThreads>
@@ -628,8 +628,11 @@ hipError_t store_of(const Fp8Cache& c, const void* key, int64_t key_stride, cons
                     const int32_t* slots, int32_t num_tokens, hipStream_t stream) {
   int lane_bits = 1;
   while ((8 << lane_bits) < c.head_dim) ++lane_bits;
-  if (c.group << lane_bits <= kStoreHold * kWave)
+  const int pieces = c.group << lane_bits;
+  if (pieces <= kStoreHold * kWave)
     return store_by<T, kWave>(c, key, key_stride, value, value_stride, slots, num_tokens, lane_bits, stream);
+  if (pieces <= kStoreHold * 2 * kWave)
+    return store_by<T, 2 * kWave>(c, key, key_stride, value, value_stride, slots, num_tokens, lane_bits, stream);
   return store_by<T, kThreads>(c, key, key_stride, value, value_stride, slots, num_tokens, lane_bits, stream);
 }
 
