@@ -478,14 +478,17 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const float* __r
 // one head of K or V, and encodes them under a scale of their own. As in the
 // cache write, a thread keeps the pieces that it read, of 16 codes here.
 
+constexpr int kCompactHold = 2;
+template <int kThreads>
 __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatch from,
                                                            const int32_t* __restrict__ indices,
                                                            const int32_t* __restrict__ counts, int32_t keep,
                                                            const int32_t* __restrict__ to_tables, int64_t to_stride,
                                                            int32_t to_width, int32_t lane_bits) {
-  constexpr int kHold = 2;
+  constexpr int kHold = kCompactHold;
   __shared__ float wave_amax[kThreads / kWave];
-  __shared__ int64_t source[kMaxGroup], source_scale[kMaxGroup];  // each row's slot, or -1, and its scale's element
+  constexpr int kRows = kThreads < 4 * kWave ? kHold * kThreads : kMaxGroup;  // fewer waves hold the group (launch_compact)
+  __shared__ int64_t source[kRows], source_scale[kRows];  // each row's slot, or -1, and its scale's element
   const int tid = threadIdx.x;
   const Slice slice = slice_of(blockIdx.x, 2 * c.heads);
   const int seq = slice.unit % from.num_seqs;
@@ -670,8 +673,14 @@ hipError_t launch_compact(const Fp8Cache& c, const PagedBatch& from, const int32
   const dim3 grid((unsigned)slices_grid((int64_t)((keep + c.group - 1) / c.group) * from.num_seqs, 2 * c.heads));
   int lane_bits = 0;
   while ((16 << lane_bits) < c.head_dim) ++lane_bits;
-  compact_kernel<<<grid, dim3(kThreads), 0, stream>>>(c, from, indices, counts, keep, to_tables, to_stride, to_width,
-                                                      lane_bits);
+  // Waves as many as hold a group, up to four (8 contexts of 8 heads cut to 2,048 tokens in groups of 16 20 us, 41 by four).
+  auto launch = [&](auto kernel, int threads) {
+    kernel<<<grid, dim3(threads), 0, stream>>>(c, from, indices, counts, keep, to_tables, to_stride, to_width, lane_bits);
+  };
+  const int pieces = c.group << lane_bits;
+  if (pieces <= kCompactHold * kWave) launch(compact_kernel<kWave>, kWave);
+  else if (pieces <= kCompactHold * 2 * kWave) launch(compact_kernel<2 * kWave>, 2 * kWave);
+  else launch(compact_kernel<kThreads>, kThreads);
   return hipGetLastError();
 }
 
