@@ -767,3 +767,25 @@ def test_blocks_of_codes_and_scales_are_saved_and_restored(gpu, layers, block, g
             assert torch.equal(got[:, :, now], want[:, :, was])
         for other in (0, 2, 4, 5):
             assert (got[:, :, other] == 0x55).all()
+
+
+@pytest.mark.parametrize("rows", [33, 64, 127, 128, 129])
+def test_weights_about_the_border_between_the_kernels(gpu, rows):
+    test_weights(gpu, [190, 300, 5, 0], [rows, 8, 5, 1], 2, 1, 128, 64, 16, torch.bfloat16)
+
+
+@pytest.mark.parametrize("lens", [[255, 256], [257, 511], [513, 1025], [2048, 1000]])
+def test_chunks_about_the_borders_of_splits(gpu, lens):
+    Setup(gpu, lens, [40, 3], 1, 4, 128, 256, 16, unused=NAN).check()
+
+
+@pytest.mark.parametrize("heads,hd,group", [(8, 128, 16), (8, 128, 32), (4, 256, 64), (16, 64, 16)])
+def test_tokens_appended_to_many_groups_at_once(gpu, heads, hd, group):
+    # More than one workgroup for each: a workgroup's tokens continue, start and skip groups of their own.
+    n, block = 500, 64
+    g = torch.Generator().manual_seed(5)
+    groups = torch.randperm(n + 7, generator=g)[:n]
+    slots = groups * group + torch.randint(0, group, (n,), generator=g)
+    slots[::9], slots[4::50] = groups[::9] * group, -1
+    caches = pool(-(-(n + 7) * group // block), block, group, heads, hd)
+    check_store(gpu, rows(n, heads, hd, torch.bfloat16, 1, 30.0), rows(n, heads, hd, torch.bfloat16, 2), caches, slots.tolist())
