@@ -337,17 +337,12 @@ def run(state):
     return {"rotary": _rotary, "store": _store, "attend": _attend, "weights": _weights, "evict": _evict}[state.kind](state)
 
 
-_ops = None  # kvx.ops, imported by the first pass
-
-
 def _run_own(s):
-    global _ops
-    if _ops is None:
-        sys.path.insert(0, str(Path.cwd() / "kv-cache-offloading_amd"))
-        from kvx import ops
+    root = str(Path.cwd() / "kv-cache-offloading_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from kvx import ops
 
-        _ops = ops
-    ops = _ops
     if s.kind == "rotary":
         return ops.rotary_embed(s.q, s.k, s.positions, s.frequencies, interleaved=s.interleaved, magnitude=s.magnitude)
     if s.kind == "store":
