@@ -341,7 +341,9 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
         if (__any(high > top[n] + 8.0f)) {  // see the chunks' kernel
           top[n] = fmaxf(rows_max(high), top[n]);
           const float now = top[n] == -INFINITY ? base[n] : ceilf(top[n]);
-          const float fade = __builtin_amdgcn_exp2f(base[n] - now);
+          // The base only rises, but for the first time, from 0, to a row's scores that may all lie below -128: nothing
+          // has been summed then, and infinity times it would be NaN.
+          const float fade = __builtin_amdgcn_exp2f(fminf(base[n] - now, 0.0f));
           base[n] = now;
           sum[n] *= fade;
 #pragma unroll
