@@ -746,9 +746,10 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       high = fmaxf(low * scale[0], high * scale[1]);
       if (__any(high > top + 8.0f)) {
         top = fmaxf(top, fmaxf(high, __shfl_xor(high, 32)));
-        // A whole number, so that `fade` is a power of two and nothing is rounded.
+        // A whole number, so that `fade` is a power of two and nothing is rounded. The base only rises, but for the first
+        // time, from 0, when nothing has been summed (as above).
         const float now_base = top == -INFINITY ? base : ceilf(top);
-        const float fade = __builtin_amdgcn_exp2f(base - now_base);
+        const float fade = __builtin_amdgcn_exp2f(fminf(base - now_base, 0.0f));
         base = now_base;
         sum *= fade;
 #pragma unroll

@@ -65,3 +65,25 @@ def test_few_rows_with_one_stretch_near_zero(gpu, hd, rows, near):
 @pytest.mark.parametrize("hd", [64, 128])
 def test_few_rows_with_low_scores_in_later_splits_alone(gpu, hd):
     check(lowered(gpu, [2100], None, 1, 4, hd, torch.bfloat16, 300, [(0, group) for group in range(64)]))
+
+
+@pytest.mark.parametrize("level", [100, 400])
+@pytest.mark.parametrize("hd,per_kv,dtype", [(64, 2, torch.bfloat16), (128, 2, torch.bfloat16), (96, 4, torch.float16),
+                                             (256, 1, torch.bfloat16)])
+def test_all_scores_of_chunks_far_below_zero(gpu, hd, per_kv, dtype, level):
+    # A whole prompt, chunks behind prefixes of less than a pass and of several, one row, more rows than tokens.
+    lens, q_lens = [40, 71, 700, 1, 3], [40, 33, 50, 1, 5]
+    lse = check(lowered(gpu, lens, q_lens, 1, per_kv, hd, dtype, level))
+    assert (lse[lse.isfinite()] < -89).all()
+
+
+@pytest.mark.parametrize("near", [0, 1, 2, 9, 70, 129])
+@pytest.mark.parametrize("hd,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (128, torch.float16)])
+def test_chunks_with_one_stretch_near_zero(gpu, hd, dtype, near):
+    # 2,100 keys in several splits; rows 0 to 35 of the chunk do not see the last groups.
+    check(lowered(gpu, [2100, 300], [40, 1], 1, 4, hd, dtype, 200, [(0, near)]))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_chunks_with_low_scores_in_later_splits_alone(gpu, hd):
+    check(lowered(gpu, [2100], [40], 1, 4, hd, torch.bfloat16, 300, [(0, group) for group in range(64)]))
