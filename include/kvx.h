@@ -212,7 +212,7 @@ typedef struct kvx_fp8_cache {
 typedef struct kvx_paged_batch {
   const int32_t* block_tables;
   const int32_t* context_lens;
-  const int32_t* cu_seqlens; /* NULL: one row a sequence */
+  const int32_t* cu_seqlens; /* NULL: one row a sequence, or none in the call (num_tokens 0) */
   int64_t table_stride;      /* elements */
   int32_t table_width;       /* blocks of a table */
   int32_t num_seqs;

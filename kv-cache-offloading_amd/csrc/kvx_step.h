@@ -174,7 +174,7 @@ struct QueryRows {
   int first, count;
 };
 __device__ __forceinline__ QueryRows query_rows(const PagedBatch& b, int seq) {
-  if (!b.cu_seqlens) return {seq, 1};
+  if (!b.cu_seqlens) return {seq, seq < b.num_tokens ? 1 : 0};  // a call may have no rows at all
   int lo = b.cu_seqlens[seq], hi = b.cu_seqlens[seq + 1];
   lo = lo < 0 ? 0 : lo > b.num_tokens ? b.num_tokens : lo;
   hi = hi < lo ? lo : hi > b.num_tokens ? b.num_tokens : hi;
