@@ -117,8 +117,27 @@ __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// 1 / s of a power of two within [2^-126, 2^126].
-__device__ __forceinline__ float reciprocal2(float s) { return __uint_as_float(0x7F000000u - __float_as_uint(s)); }
+__device__ __forceinline__ bool is_power_of_two(float s) { return (__float_as_uint(s) & 0x7FFFFFu) == 0; }  // for s >= 2^-126
+
+// For the fp32 number q nearest to q + rest: a neighbour of q + rest whose last bit is set, where rest is not 0. Rounded to
+// the 4 bits of a code, that gives what q + rest itself gives; q, which may have become halfway between two codes, does not.
+__device__ __forceinline__ float to_odd(float q, float rest) {
+  const uint32_t u = __float_as_uint(q);
+  if (!(rest < 0.0f || rest > 0.0f) || (u & 1) || q == 0.0f) return q;
+  return __uint_as_float((rest > 0.0f) == (q > 0.0f) ? u + 1 : u - 1);
+}
+
+// x / s, and code * times, to odd. Scales are a user's own where they are no powers of two.
+__device__ __forceinline__ float quotient_odd(float x, float s) {
+  // Both within range of one another, so that the remainder is exact where x / s is no code of 0.
+  const int e = (int)(__float_as_uint(s) >> 23) - 127;
+  const float y = __builtin_amdgcn_ldexpf(x, -e), m = __builtin_amdgcn_ldexpf(s, -e), q = y / m;
+  return to_odd(q, __builtin_fmaf(-q, m, y));
+}
+__device__ __forceinline__ float product_odd(float code, float times) {
+  const float q = code * times;
+  return to_odd(q, __builtin_fmaf(code, times, -q));
+}
 
 // Four fp32 -> four e4m3 codes, to nearest even. Infinities saturate at +-448, NaN stays NaN.
 __device__ __forceinline__ float clamp448(float x) { return x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x; }

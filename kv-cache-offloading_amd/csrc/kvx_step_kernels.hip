@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
     for (int w = 0; w < kThreads / kWave; ++w) amax = fmaxf(amax, wave_amax[w]);
     const float kept = owner[0] < 0 && scale_before > 0.0f && scale_before < INFINITY ? scale_before : 0.0f;
     const float fit = fmaxf(scale_for(amax), kept), inverse = 1.0f / fit, shrink = kept / fit;
-    const bool grew = kept > 0.0f && fit > kept;
+    const bool grew = kept > 0.0f && fit > kept, power = is_power_of_two(fit);
     if (tid == 0) *scale = fit;
     uint8_t* codes = (is_v ? c.v : c.k) + ((int64_t)slot_base * c.heads + head) * c.head_dim + at;
     auto write = [&](int row, const Eight<T>* held_row) {
@@ -279,11 +279,17 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
       float x[8];
       if (token >= 0) {
         expand<T>(held_row ? *held_row : *reinterpret_cast<const Eight<T>*>(src + token * src_stride + at), x);
-        *dst = encode8(x, inverse);
+        if (!power) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = quotient_odd(x[j], fit);
+        }
+        *dst = encode8(x, power ? inverse : 1.0f);
       } else if (grew && row < c.group && in_row) {
         decode4(dst->x, x);
         decode4(dst->y, x + 4);
-        *dst = encode8(x, shrink);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = product_odd(x[j], shrink);
+        *dst = encode8(x, 1.0f);
       }
     };
 #pragma unroll

@@ -29,3 +29,73 @@ def test_no_rows_for_sequences_that_have_tokens(gpu, monkeypatch, native, per_kv
     mine = before.clone()
     assert torch.equal(ops.attention_weights_fp8(*args, weights=mine), before)
     assert (ops.attention_weights_fp8(*args) == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# Scales that are no powers of two: a user's own, which a group that goes on keeps.
+
+def nearest(x):
+    """float64 -> e4m3 codes by one rounding, ties to even: steps of 1/8 of the leading bit, 2^-9 below 2^-6."""
+    x = x.clamp(-448.0, 448.0)
+    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(2.0 ** -20))).clamp_min(-6.0) - 3)
+    return (torch.round(x / step) * step).float().to(ref.FP8).view(torch.uint8)
+
+
+def borders():
+    """The 126 values halfway between neighbouring finite codes, as float64."""
+    values = ref.decode(torch.arange(0x7F, dtype=torch.uint8))
+    return (values[1:] + values[:-1]) / 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd,group", [(128, 16), (64, 64), (256, 128)])
+def test_codes_are_nearest_under_a_kept_scale_of_any_value(gpu, hd, group, dtype):
+    """The quotients of fp32 rows fall on the borders between codes and next to them, where x times 1 / s, and a quotient
+    rounded to fp32 before it is rounded to a code, come out on the wrong side."""
+    heads, blocks = 2, 6
+    g = torch.Generator().manual_seed(group)
+    codes, _ = ref.random_cache(blocks, group, group, heads, hd, 1)
+    scales = ((torch.rand((blocks, 1, heads, 1), generator=g) + 0.5)
+              * torch.randint(-30, 30, (blocks, 1, heads, 1), generator=g).float().exp2())
+    n = 15  # tokens 1 .. 15 of each block's first group
+    pick = borders()[torch.randint(0, 126, (blocks, n, heads, hd), generator=g)]
+    x = (pick * scales.double()).float()
+    up = torch.nextafter(x, torch.full_like(x, torch.inf))
+    down = torch.nextafter(x, torch.zeros_like(x))
+    x = torch.stack([x, up, down])[torch.randint(0, 3, (1, *x.shape), generator=g), torch.arange(blocks)[:, None, None, None],
+                                   torch.arange(n)[:, None, None], torch.arange(heads)[:, None], torch.arange(hd)][0]
+    x = x * (torch.randint(0, 2, x.shape, generator=g) * 2 - 1)
+    limit = 448.0 * torch.exp2(torch.floor(torch.log2(scales)))  # up to here no larger power of two is asked for
+    x = x.clamp(-limit, limit).to(dtype)
+    slots = (torch.arange(blocks)[:, None] * group + torch.arange(1, n + 1)).flatten()
+    want = codes.clone()
+    want[:, 1:n + 1] = nearest(x.double() / scales.double())
+    kc, vc, ks, vs = fp8(codes, gpu), fp8(codes, gpu), scales.to(gpu), scales.clone().to(gpu)
+    rows = x.flatten(0, 1).to(gpu)
+    ops.store_kvcache_fp8(rows, -rows, kc, vc, ks, vs, slots.int().to(gpu))
+    assert torch.equal(ks.cpu(), scales) and torch.equal(vs.cpu(), scales)
+    assert torch.equal(kc.view(torch.uint8).cpu(), want)
+    want[:, 1:n + 1] = nearest(-x.double() / scales.double())
+    assert torch.equal(vc.view(torch.uint8).cpu(), want)
+
+
+@pytest.mark.parametrize("hd,group", [(128, 16), (64, 64)])
+def test_codes_are_nearest_where_a_scale_of_any_value_grows(gpu, hd, group):
+    """Old codes under a kept scale that makes some of them fall next to the border between two new ones."""
+    heads, blocks = 2, 40
+    g = torch.Generator().manual_seed(5)
+    codes, _ = ref.random_cache(blocks, group, group, heads, hd, 1)
+    aim = borders()[torch.randint(40, 110, (blocks, 1, heads, 1), generator=g)]
+    held = ref.decode(torch.randint(60, 0x7F, aim.shape, generator=g, dtype=torch.uint8))
+    scales = (aim / held).float()  # held * scale is nearly a border under a scale of 1
+    while (scales >= 1).any():
+        scales = torch.where(scales >= 1, scales / 2, scales)
+    scales = torch.stack([scales, torch.nextafter(scales, scales * 2)])[torch.randint(0, 2, (1,), generator=g)][0]
+    x = torch.full((blocks, heads, hd), 300.0, dtype=torch.bfloat16)  # asks for a scale of 1
+    slots = torch.arange(blocks) * group + 3
+    want = nearest(ref.decode(codes) * scales.double())
+    want[:, 3] = nearest(x.double())
+    kc, vc, ks, vs = fp8(codes, gpu), fp8(codes, gpu), scales.to(gpu), scales.clone().to(gpu)
+    ops.store_kvcache_fp8(x.to(gpu), x.to(gpu), kc, vc, ks, vs, slots.int().to(gpu))
+    assert (ks == 1).all() and (vs == 1).all()
+    assert torch.equal(kc.view(torch.uint8).cpu(), want) and torch.equal(vc.view(torch.uint8).cpu(), want)
