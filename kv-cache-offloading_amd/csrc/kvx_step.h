@@ -106,14 +106,16 @@ hipError_t launch_compact(const Fp8Cache& c, const PagedBatch& from, const int32
 // ---------------------------------------------------------------------------
 // Device helpers
 
-// The least power of two s >= 2^-100 with amax / s <= 448 = 0.875 * 2^9, for a
+// The least power of two s >= 2^-100 with 2^kUp amax / s <= 448 = 0.875 * 2^9, for a
 // finite amax >= 0. A power of two costs e4m3, itself a floating format, no
 // precision, makes x / s and the requantisation of codes exact but for e4m3's
 // own rounding, and lets no order of writes change a group's scale.
+template <int kUp = 0>
 __device__ __forceinline__ float scale_for(float amax) {
   const uint32_t u = __float_as_uint(amax);
-  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  int e = (int)(u >> 23) - 127 - 8 + kUp + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   e = e < -100 ? -100 : e;
+  if (kUp > 0 && e > 127) e = 127;
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 

@@ -552,18 +552,15 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
     }
     return r;
   };
-  auto value = [&](const Row& r, float* x) {
+  // The largest finite code's value, over 2^10: the value itself may exceed fp32 (256 under a scale of 2^120, which a bf16
+  // value of nearly 2^128 is stored as). Rounded to odd, so that it lies on its own side of the border between two scales.
+  auto amax_of = [&](const Row& r) {
+    float x[16], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) decode4(r.codes[i], x + 4 * i);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= r.scale;
-  };
-  auto amax_of = [&](const Row& r) {
-    float x[16], most = 0.0f;
-    value(r, x);
-#pragma unroll
     for (int i = 0; i < 16; ++i) most = fmaxf(most, finite_abs(x[i]));
-    return most;
+    return finite_abs(product_odd(most * 0x1p-10f, r.scale));
   };
   Row held[kHold];
   float amax = 0.0f;
@@ -577,14 +574,23 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Fp8Cache c, PagedBatc
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / kWave; ++w) amax = fmaxf(amax, wave_amax[w]);
-  const float fit = scale_for(amax), inverse = 1.0f / fit;
+  const float fit = scale_for<10>(amax), inverse = 1.0f / fit;
   if (tid == 0)
     scales[((int64_t)target * (c.block_size / c.group) + c.group_of(first - to_block * c.block_size)) * c.heads + head] = fit;
   auto write = [&](const Row& r, int row) {
     if (row >= rows || !in_row) return;
     float x[16];
-    value(r, x);
-    const u32x2 lo = encode8(x, inverse), hi = encode8(x + 8, inverse);
+    const float times = r.scale * inverse;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) decode4(r.codes[i], x + 4 * i);
+    if (is_power_of_two(r.scale)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= times;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = product_odd(x[i], times);
+    }
+    const u32x2 lo = encode8(x, 1.0f), hi = encode8(x + 8, 1.0f);
     *reinterpret_cast<u32x4*>(codes + ((to_slot + row) * c.heads + head) * c.head_dim + at) = u32x4{lo.x, lo.y, hi.x, hi.y};
   };
 #pragma unroll

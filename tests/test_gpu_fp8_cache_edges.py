@@ -99,3 +99,48 @@ def test_codes_are_nearest_where_a_scale_of_any_value_grows(gpu, hd, group):
     ops.store_kvcache_fp8(x.to(gpu), x.to(gpu), kc, vc, ks, vs, slots.int().to(gpu))
     assert (ks == 1).all() and (vs == 1).all()
     assert torch.equal(kc.view(torch.uint8).cpu(), want) and torch.equal(vc.view(torch.uint8).cpu(), want)
+
+
+def compacted(gpu, codes, scales, block):
+    """Blocks 0 .. n - 1 moved whole to n .. 2n - 1, in the order of the last row of each block first: codes and scales."""
+    n, heads = codes.shape[0], codes.shape[2]
+    twice = [torch.cat([t, torch.zeros_like(t)]) for t in (codes, scales)]
+    kc, vc, ks, vs = fp8(twice[0], gpu), fp8(twice[0], gpu), twice[1].to(gpu), twice[1].clone().to(gpu)
+    tables = torch.arange(n, dtype=torch.int32)[:, None]
+    order = torch.arange(block - 1, -1, -1, dtype=torch.int32).repeat(n, heads, 1)
+    ops.compact_kvcache_fp8(kc, vc, ks, vs, tables.to(gpu), order.to(gpu), int32([block] * n, gpu), (tables + n).to(gpu))
+    assert torch.equal(kc.view(torch.uint8), vc.view(torch.uint8)) and torch.equal(ks, vs)
+    return kc[n:].view(torch.uint8).cpu(), ks[n:].cpu()
+
+
+@pytest.mark.parametrize("hd,group", [(128, 16), (64, 64), (256, 128)])
+def test_compacted_codes_are_nearest_under_scales_of_any_value(gpu, hd, group):
+    heads, blocks, block = 2, 20, 2 * group
+    g = torch.Generator().manual_seed(5)
+    codes, _ = ref.random_cache(blocks, block, group, heads, hd, 1)
+    shape = (blocks, 2, heads, 1)
+    aim = borders()[torch.randint(40, 110, shape, generator=g)]
+    held = ref.decode(torch.randint(60, 0x7F, shape, generator=g, dtype=torch.uint8))
+    scales = (aim / held).float()  # held * scale is nearly a border under each power of two
+    # Codes whose value is the most that a scale holds, nearly: 448 s, and s a little more or less than a power of two.
+    codes[::3, :group, 0, 3] = 0x7E
+    scales[::3, 0, 0, 0] = torch.nextafter(torch.tensor(1.0), torch.tensor([2.0, 0.0])[torch.randint(0, 2, (7,), generator=g)])
+    value = (ref.decode(codes) * scales.double().repeat_interleave(group, 1)).flip(1)
+    want_scale = torch.tensor([[[[ref.least_scale(float(value[b, i * group:(i + 1) * group, h].abs().max()))]
+                                 for h in range(heads)] for i in range(2)] for b in range(blocks)])
+    got, got_scale = compacted(gpu, codes, scales, block)
+    assert torch.equal(got_scale.double(), want_scale.double())
+    assert torch.equal(got, nearest(value / want_scale.double().repeat_interleave(group, 1)))
+
+
+def test_the_largest_values_are_compacted(gpu):
+    """Codes of 256 and more under a scale of 2^120, as the largest bf16 values are stored, stand for more than fp32 holds."""
+    block, heads, hd = 16, 2, 64
+    codes, _ = ref.random_cache(4, block, 16, heads, hd, 1)
+    codes[0, 3, 0, 5], codes[1, 9, 1, 7], codes[2] = 0x78, 0xFE, codes[2] & 0x77
+    scales = torch.tensor([2.0 ** 120, 2.0 ** 120, 2.0 ** 120, 2.0 ** -100]).view(4, 1, 1, 1).repeat(1, 1, heads, 1)
+    tables, indices = torch.arange(4)[:, None].int(), torch.arange(block).repeat(4, heads, 1).int()
+    twice = [torch.cat([t, torch.zeros_like(t)]) for t in (codes, scales)]
+    want, want_scale = ref.compact(*twice, tables, indices.flip(2), torch.tensor([block] * 4), tables + 4)
+    got, got_scale = compacted(gpu, codes, scales, block)
+    assert torch.equal(got_scale, want_scale[4:]) and torch.equal(got, want[4:])
