@@ -144,3 +144,25 @@ def test_the_largest_values_are_compacted(gpu):
     want, want_scale = ref.compact(*twice, tables, indices.flip(2), torch.tensor([block] * 4), tables + 4)
     got, got_scale = compacted(gpu, codes, scales, block)
     assert torch.equal(got_scale, want_scale[4:]) and torch.equal(got, want[4:])
+
+
+# ---------------------------------------------------------------------------
+# The second product's weights, in 16 bits
+
+BITS_16 = 2.0 ** -16  # two roundings to bf16, the second of the first one's remainder: half a step, 2^-8, of 2^-8
+
+
+@pytest.mark.parametrize("hd,per_kv,q_lens,dtype", [
+    (128, 4, None, torch.bfloat16), (64, 8, [1, 4, 4, 3], torch.bfloat16), (256, 2, [2, 20, 7, 1], torch.bfloat16),
+    (128, 4, [1, 40, 33, 8], torch.bfloat16), (64, 2, [1, 70, 33, 8], torch.bfloat16), (112, 3, [1, 40, 33, 8], torch.bfloat16),
+    (128, 4, None, torch.float16), (128, 4, [1, 40, 33, 8], torch.float16), (64, 2, [1, 70, 33, 8], torch.float16)])
+@pytest.mark.parametrize("powers", [True])
+def test_the_weights_of_the_values_keep_16_bits(gpu, hd, per_kv, q_lens, dtype, powers):
+    """Few rows and chunks, in both types, under any scales: outputs near 0, where the values cancel out, show it."""
+    Setup(gpu, [33, 90, 300, 2100], q_lens, 2, per_kv, hd, 64, 32, dtype, powers=powers).check(p_step=BITS_16)
+
+
+def test_rows_do_not_change_their_precision_with_the_hint(gpu):
+    s = Setup(gpu, [200, 300], [150, 33], 1, 4, 64, 32, 32)
+    for most in (1, 8, 16, 150, 183):  # the first two by the kernel of few rows, whose sequences may be longer
+        s.check(p_step=BITS_16, max_seqlen=most)
