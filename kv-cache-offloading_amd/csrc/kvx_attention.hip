@@ -478,9 +478,10 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 // over the keys kKeys at a time. The waves convert the codes
 // to bf16 (K: the query's type) into LDS once for all of them: K's rows as they
 // are, V transposed, with the exponent of its scale applied by the converting
-// instruction. LDS is double-buffered, the codes of the next keys are loaded
-// into registers while the present ones are used, and their blocks are looked
-// up one pass before that.
+// instruction (what a user's own scale is besides, P takes: rounded into V, it
+// would leave V 8 bits). LDS is double-buffered, the codes of the next keys are
+// loaded into registers while the present ones are used, and their blocks are
+// looked up one pass before that.
 // As above, S^T = K Q^T and O^T = V^T P^T, now by mfma 32x32x16: lane (n, h), n =
 // lane % 32, h = lane / 32, gets query row n's scores of keys 8 (i / 4) + 4 h + i % 4;
 // V^T's rows in LDS hold the keys in the order in which P lies in the lanes.
@@ -504,6 +505,11 @@ __device__ __forceinline__ f32x16 mfma32(typename Query<kType>::Vec a, typename 
 __device__ __forceinline__ uint32_t pair_scaled(uint32_t codes, float scale, bool high) {
   return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+}
+
+// A scale over its power of two, within [1, 2).
+__device__ __forceinline__ float rest_of(float scale) {
+  return __uint_as_float((__float_as_uint(scale) & 0x007FFFFFu) | 0x3F800000u);
 }
 
 // What a pass needs to know of its keys' 16-key tiles.
@@ -675,7 +681,6 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       for (int i = 0; i < kVLoads; ++i) {
         const unsigned group = (i * kThreads + wave * kWave + lane) / kVThreads, col = lane % kVThreads * kVCols;
         const float scale = kVUniform ? scalar(from.v_scale[(i * kThreads + wave * kWave) / kVThreads / 2]) : from.v_scale[group / 2];
-        const float rest = __uint_as_float((__float_as_uint(scale) & 0x007FFFFFu) | 0x3F800000u);  // in [1, 2)
         if (masked) {
           uint32_t nan = 0;
 #pragma unroll
@@ -695,14 +700,8 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         uint8_t* to = v_to + col * kVRow + ((group ^ (col / 16 % 4)) * 16);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          u32x4 w = {pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
-                     pair_scaled(hi[d], scale, false), pair_scaled(hi[d], scale, true)};
-          if (rest != 1.0f) {  // no power of two: the rest of the scale costs V one rounding to bf16
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              w[j] = pack_bf16(__uint_as_float(w[j] << 16) * rest, __uint_as_float(w[j] & 0xFFFF0000u) * rest);
-          }
-          *reinterpret_cast<u32x4*>(to + d * kVRow) = w;
+          *reinterpret_cast<u32x4*>(to + d * kVRow) = u32x4{pair_scaled(lo[d], scale, false), pair_scaled(lo[d], scale, true),
+                                                            pair_scaled(hi[d], scale, false), pair_scaled(hi[d], scale, true)};
         }
       }
     };
@@ -719,6 +718,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
     // output. Operands are read kAhead products ahead. The scheduling barriers keep it so: left alone, the compiler
     // waits for each operand right before its product.
     float tile_scale = 0.0f;   // lane l: of the pass's tile l
+    bool own_scales = false;   // some of V's in the pass are no powers of two
     uint32_t tiles_there = 0;  // bit l: whether tile l is in a block
     constexpr int kAhead = 2;
     Vec k_next[kAhead + 1];
@@ -766,6 +766,16 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       auto read_v = [&](int t) {
         v_next[t % (kAhead + 1)] = *reinterpret_cast<const bf16x8*>(v_at(buffer, step, t / kOuts, t % kOuts));
       };
+      // P takes what is left of V's scales through its exponents, and its sum goes without.
+      float from[2] = {-base, -base}, over[2] = {1.0f, 1.0f}, part[2] = {0.0f, 0.0f};
+      if (own_scales) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float rest = rest_of(scalar(info[pass & 3].v_scale[step * 2 + i]));
+          from[i] += __builtin_amdgcn_logf(rest);
+          over[i] = __builtin_amdgcn_rcpf(rest);
+        }
+      }
       u32x4 p[2][2];  // P to bf16, and what the rounding left
       // The wave that has scores and exponentials to issue goes first, so that the SIMD's two waves fall out of step and
       // one's outputs run under the other's exponentials: 477 us in place of 511 for two chunks behind 6-8 K tokens.
@@ -780,15 +790,17 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
         }
 #pragma unroll
         for (int i = t * kEach; i < (t + 1) * kEach; ++i) {
-          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], scale[i / 4], -base));
-          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], scale[i / 4], -base));
-          sum += e0 + e1;
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], scale[i / 4], from[i / 4]));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], scale[i / 4], from[i / 4]));
+          part[i / 4] += e0 + e1;
           const uint32_t hi = pack_bf16(e0, e1);
           p[0][i / 4][i % 4] = hi;
           p[1][i / 4][i % 4] = pack_bf16(e0 - __uint_as_float(hi << 16), e1 - __uint_as_float(hi & 0xFFFF0000u));
         }
         if (kMore) __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum = __builtin_fmaf(part[i], over[i], sum);
       if (!kMore) {
 #pragma unroll
         for (int t = 0; t < kAhead; ++t) read_v(t);
@@ -834,6 +846,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
 #pragma unroll
         for (int d = 0; d < kDots; ++d) x = mfma32<kType>(*reinterpret_cast<const Vec*>(k_at(buffer, 0) + d * 32), q[d], x);
         tile_scale = now.k_scale[lane % kTiles16];
+        own_scales = __any(rest_of(now.v_scale[lane % kTiles16]) != 1.0f);
         tiles_there = (uint32_t)__ballot(now.row[lane % kTiles16] >= 0);
 #pragma unroll
         for (int t = 0; t < kAhead; ++t) read_k(buffer, 1, t);

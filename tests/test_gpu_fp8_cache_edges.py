@@ -156,7 +156,7 @@ BITS_16 = 2.0 ** -16  # two roundings to bf16, the second of the first one's rem
     (128, 4, None, torch.bfloat16), (64, 8, [1, 4, 4, 3], torch.bfloat16), (256, 2, [2, 20, 7, 1], torch.bfloat16),
     (128, 4, [1, 40, 33, 8], torch.bfloat16), (64, 2, [1, 70, 33, 8], torch.bfloat16), (112, 3, [1, 40, 33, 8], torch.bfloat16),
     (128, 4, None, torch.float16), (128, 4, [1, 40, 33, 8], torch.float16), (64, 2, [1, 70, 33, 8], torch.float16)])
-@pytest.mark.parametrize("powers", [True])
+@pytest.mark.parametrize("powers", [True, False])
 def test_the_weights_of_the_values_keep_16_bits(gpu, hd, per_kv, q_lens, dtype, powers):
     """Few rows and chunks, in both types, under any scales: outputs near 0, where the values cancel out, show it."""
     Setup(gpu, [33, 90, 300, 2100], q_lens, 2, per_kv, hd, 64, 32, dtype, powers=powers).check(p_step=BITS_16)
