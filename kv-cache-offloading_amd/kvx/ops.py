@@ -21,6 +21,8 @@ from kvx._lib import bind as _bind
 FORMAT_RAW, FORMAT_FP8 = _lib.FORMAT_RAW, _lib.FORMAT_FP8
 SCALE_DTYPES = {torch.bfloat16: _lib.SCALE_BF16, torch.float32: _lib.SCALE_FP32}
 
+_INT32_MAX = 2 ** 31 - 1  # what ctypes would cut larger numbers to, without an error
+
 # Largest finite float8_e4m3fn magnitude (the codec's clamp bound).
 FP8_MAX = 448.0
 
@@ -446,12 +448,14 @@ def _paged_batch(block_tables: torch.Tensor, context_lens: torch.Tensor, cu_seql
             (block_tables.numel() and block_tables.stride(1) != 1 and block_tables.shape[1] > 1):
         raise TypeError("block_tables must be an int32 [sequences, blocks] tensor with contiguous rows")
     seqs, width = block_tables.shape
+    if max(seqs, width, num_tokens) > _INT32_MAX:
+        raise NotImplementedError("more than 2^31 sequences, blocks or query rows in one call")
     if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) or not context_lens.is_contiguous():
         raise TypeError("context_lens must be a contiguous int32 tensor, one for each sequence")
     if cu_seqlens is not None:
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (seqs + 1,) or not cu_seqlens.is_contiguous():
             raise TypeError("cu_seqlens must be a contiguous int32 tensor of sequences + 1")
-        max_seqlen = num_tokens if max_seqlen is None else max_seqlen
+        max_seqlen = num_tokens if max_seqlen is None else min(max_seqlen, num_tokens)
     else:
         if max_seqlen not in (None, 1):
             raise ValueError("without cu_seqlens each sequence has one query row: max_seqlen is 1")
@@ -618,6 +622,9 @@ def select_tokens(weights: torch.Tensor, context_lens: torch.Tensor, keep: int,
         raise TypeError("context_lens must be a contiguous int32 tensor, one for each sequence")
     if keep < 0 or recent < 0 or heads == 0:
         raise ValueError("keep and recent must be non-negative, and heads at least 1")
+    if keep > _INT32_MAX:
+        raise NotImplementedError(f"select_tokens keeps at most {_INT32_MAX} tokens (got {keep})")
+    recent = min(recent, keep)
     device = _require_device(weights, context_lens)
     indices = torch.empty((seqs, heads, keep), dtype=torch.int32, device=device)
     counts = torch.empty((seqs,), dtype=torch.int32, device=device)

@@ -230,3 +230,12 @@ def test_scaled_frequencies():
 def test_frequencies_refused(args, match):
     with pytest.raises(ValueError, match=match):
         ops.rotary_frequencies(*args, device="cpu")
+
+
+def test_numbers_past_32_bits_are_not_cut_to_them():
+    with pytest.raises(NotImplementedError, match="at most"):
+        ops.select_tokens(torch.zeros((3, 2, 9)), LENS, 2 ** 32 + 1)
+    cu = torch.tensor([0, 1, 2, 5], dtype=torch.int32)
+    assert ops._paged_batch(TABLES, LENS, cu, 2 ** 32 + 2, 5).max_seqlen == 5  # a hint: no sequence has more than all rows
+    with pytest.raises(NotImplementedError, match="rows in one call"):
+        ops._paged_batch(TABLES, LENS, cu, None, 2 ** 32 + 1)

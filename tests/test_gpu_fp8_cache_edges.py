@@ -166,3 +166,15 @@ def test_rows_do_not_change_their_precision_with_the_hint(gpu):
     s = Setup(gpu, [200, 300], [150, 33], 1, 4, 64, 32, 32)
     for most in (1, 8, 16, 150, 183):  # the first two by the kernel of few rows, whose sequences may be longer
         s.check(p_step=BITS_16, max_seqlen=most)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("recent", [5, 9, 2 ** 31, 2 ** 32 + 1])
+def test_more_recent_tokens_than_are_kept(gpu, monkeypatch, native, recent):
+    from kvx import _lib
+
+    monkeypatch.setattr(_lib, "_bind", _lib.load_bind() if native else _lib._NoBind)
+    weights = torch.rand((2, 2, 40), generator=torch.Generator().manual_seed(1))
+    got = ops.select_tokens(weights.to(gpu), int32([40, 7], gpu), 5, recent)
+    for a, b in zip(got, ref.select(weights, [40, 7], 5, recent)):
+        assert torch.equal(a.cpu(), b)
