@@ -22,6 +22,7 @@
 // as far from the formula's as their type's rounding alone leaves them, 0.0017.
 // (By one operand, 8 bits, two chunks of 3,549 rows of 32 heads take 476 us in
 // place of 590, and are 0.0023 off.)
+#include <algorithm>
 #include <type_traits>
 
 #include "kvx_step.h"
@@ -1316,7 +1317,8 @@ hipError_t attention_typed(const AttentionArgs& a, hipStream_t stream) {
     }
   }
   if (err != hipSuccess || a.splits == 1) return err;
-  const dim3 grid((unsigned)((int64_t)a.batch.max_seqlen * a.q_heads), (unsigned)a.batch.num_seqs);
+  const int64_t rows_joined = std::min<int64_t>((int64_t)a.batch.max_seqlen * a.q_heads, 1 << 20);  // others follow these
+  const dim3 grid((unsigned)rows_joined, (unsigned)a.batch.num_seqs);
   if (a.splits <= 16) join_kernel<T, 256><<<grid, dim3(256), 0, stream>>>(a);
   else join_kernel<T, 1024><<<grid, dim3(1024), 0, stream>>>(a);
   return hipGetLastError();
@@ -1360,12 +1362,16 @@ hipError_t weights_sized(const WeightsArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+constexpr int64_t kMostTiles = 1 << 18;
 AttentionPlan attention_plan(const Fp8Cache& c, const PagedBatch& b, int32_t q_heads) {
   const int64_t rows = (int64_t)b.max_seqlen * (q_heads / c.heads);
   const bool few = rows <= kFewRows || padded_head(c.head_dim) == 256;
   const int64_t tile_rows = few ? 16 * few_tiles(rows, padded_head(c.head_dim)) : 32 * kChunkWaves;
   AttentionPlan plan;
-  plan.row_tiles = (int32_t)((rows + tile_rows - 1) / tile_rows);
+  // As many tiles of rows as the longest sequence may have, but no more workgroups than keep 256 CUs busy for a thousand
+  // rounds: max_seqlen may be all rows of a call of many short sequences, and workgroups take the tiles behind theirs.
+  const int64_t room = std::max<int64_t>(kMostTiles / ((int64_t)b.num_seqs * c.heads), 1);
+  plan.row_tiles = (int32_t)std::min((rows + tile_rows - 1) / tile_rows, room);
   const int64_t groups = (int64_t)b.num_seqs * c.heads * plan.row_tiles;
   const int64_t steps = ((int64_t)b.table_width * c.block_size + kStep - 1) / kStep;
   // Split the keys while there are too few workgroups to fill the chip, each keeping 256 keys or more (1,024: 16 chunks of

@@ -224,8 +224,7 @@ int kvx_attention_fp8(const kvx_fp8_cache* cache, const kvx_paged_batch* batch, 
     return set_error(KVX_E_INVALID, "attention needs %lld bytes of workspace on 16 bytes (got %lld)", (long long)need,
                      (long long)workspace_bytes);
   a.partial = (float*)workspace;
-  if (slices_grid((int64_t)a.batch.num_seqs * a.splits * a.row_tiles, a.cache.heads) > kMostGrid / 2 ||
-      (int64_t)a.batch.max_seqlen * query_heads > kMostGrid)
+  if (slices_grid((int64_t)a.batch.num_seqs * a.splits * a.row_tiles, a.cache.heads) > kMostGrid / 2)
     return set_error(KVX_E_UNSUPPORTED, "too many sequences, heads and queries for one launch");
   return hip_status(launch_attention(a, dtype, (hipStream_t)stream), "attention_fp8 launch");
 }

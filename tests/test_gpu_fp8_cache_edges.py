@@ -178,3 +178,33 @@ def test_more_recent_tokens_than_are_kept(gpu, monkeypatch, native, recent):
     got = ops.select_tokens(weights.to(gpu), int32([40, 7], gpu), 5, recent)
     for a, b in zip(got, ref.select(weights, [40, 7], 5, recent)):
         assert torch.equal(a.cpu(), b)
+
+
+def test_many_sequences_of_one_row_without_a_hint(gpu):
+    """max_seqlen defaults to all rows, 4,100 of them for each of as many sequences."""
+    n, heads, hd = 4100, 8, 144
+    k, ks = ref.random_cache(300, 16, 16, heads, hd, 1)
+    v, vs = ref.random_cache(300, 16, 16, heads, hd, 2)
+    g = torch.Generator().manual_seed(3)
+    tables = torch.randint(0, 300, (n, 1), generator=g, dtype=torch.int32).to(gpu)
+    lens = torch.randint(0, 17, (n,), generator=g, dtype=torch.int32).to(gpu)
+    q = torch.randn((n, heads, hd), generator=g).to(torch.bfloat16).to(gpu)
+    args = (q, fp8(k, gpu), fp8(v, gpu), ks.to(gpu), vs.to(gpu), tables, lens)
+    want = ops.attention_fp8(*args, return_lse=True)
+    got = ops.attention_fp8(*args, return_lse=True, cu_seqlens=torch.arange(n + 1, dtype=torch.int32, device=gpu))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_many_rows_and_heads_without_a_hint(gpu):
+    n, rows, heads, hd = 1000, 70, 256, 16
+    k, ks = ref.random_cache(50, 80, 16, 1, hd, 1)
+    v, vs = ref.random_cache(50, 80, 16, 1, hd, 2)
+    g = torch.Generator().manual_seed(3)
+    tables = torch.randint(0, 50, (n, 1), generator=g, dtype=torch.int32).to(gpu)
+    lens = torch.randint(60, 81, (n,), generator=g, dtype=torch.int32).to(gpu)
+    q = torch.randn((n * rows, heads, hd), device=gpu).to(torch.bfloat16)
+    args = (q, fp8(k, gpu), fp8(v, gpu), ks.to(gpu), vs.to(gpu), tables, lens)
+    cu = torch.arange(n + 1, dtype=torch.int32, device=gpu) * rows
+    want = ops.attention_fp8(*args, return_lse=True, cu_seqlens=cu, max_seqlen=rows)
+    got = ops.attention_fp8(*args, return_lse=True, cu_seqlens=cu)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
