@@ -208,3 +208,61 @@ def test_many_rows_and_heads_without_a_hint(gpu):
     want = ops.attention_fp8(*args, return_lse=True, cu_seqlens=cu, max_seqlen=rows)
     got = ops.attention_fp8(*args, return_lse=True, cu_seqlens=cu)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_a_captured_step_of_all_operators_replays(gpu, rows):
+    """Rotary positions, write, attention, weights, choice and compaction in one graph, replayed as a context grows, with
+    eager work between the replays; each against the same calls made one by one on tensors of their own."""
+    heads, per_kv, hd, block, group, keep, width = 2, 4, 64, 64, 16, 20, 256
+    g = torch.Generator().manual_seed(rows)
+
+    def state():
+        codes = torch.zeros((2, 12, block, heads, hd), dtype=torch.uint8, device=gpu).view(torch.float8_e4m3fn)
+        return (codes, torch.ones((2, 12, block // group, heads, 1), device=gpu), torch.zeros((2, heads, width), device=gpu))
+
+    tables, new = int32([[3, 1, 4, 0], [5, 9, 2, 6]], gpu), int32([[7], [8]], gpu)
+    frequencies, magnitude = ops.rotary_frequencies(hd)
+    qkv = torch.zeros((2 * rows, heads * (per_kv + 2), hd), dtype=torch.bfloat16, device=gpu)
+    positions = torch.zeros(2 * rows, dtype=torch.int64, device=gpu)
+    slots, lens, cu = (torch.zeros(n, dtype=torch.int32, device=gpu) for n in (2 * rows, 2, 3))
+
+    def step(codes, scales, weights):
+        q, k = ops.rotary_embed(qkv[:, :heads * per_kv], qkv[:, heads * per_kv:-heads], positions, frequencies, magnitude=magnitude)
+        cache = (codes[0], codes[1], scales[0], scales[1])
+        ops.store_kvcache_fp8(k, qkv[:, -heads:], *cache, slots)
+        how = {} if rows == 1 else dict(cu_seqlens=cu, max_seqlen=rows)
+        out, lse = ops.attention_fp8(q, *cache, tables, lens, return_lse=True, **how)
+        ops.attention_weights_fp8(q, lse, codes[0], scales[0], tables, lens, weights=weights, **how)
+        chosen = ops.select_tokens(weights, lens, keep, 4)
+        ops.compact_kvcache_fp8(*cache, tables, chosen[0], chosen[1], new)
+        return (out, lse, *chosen)
+
+    def bits(outputs, kept):
+        return [t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (*outputs, *kept)]
+
+    mine, eager = state(), state()
+    slots.fill_(-1)
+    step(*state())  # the library is loaded
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = step(*mine)
+    length = 0
+    for _ in range(5):
+        n = rows if length else max(1, rows - 3)  # the first step's last rows are none: slots of -1, and they see what is there
+        length += n
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        at = torch.full((2, rows), -1, dtype=torch.int64)
+        at[:, :n] = torch.arange(length - n, length)
+        positions.copy_(at.clamp_min(0).flatten())
+        cpu = tables.cpu().long()
+        slot = torch.where(at >= 0, cpu.gather(1, at.clamp_min(0) // block) * block + at % block, -1)
+        slots.copy_(slot.flatten())
+        lens.fill_(length)
+        cu.copy_(torch.tensor([0, rows, 2 * rows]))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(*eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(bits(outputs, mine), bits(want, eager)))
+        assert not want[0].isnan().any()
