@@ -184,6 +184,8 @@ int kvx_scatter_tokens_fp8(void* pool, const kvx_block_layout* layout, const int
  * of 16, at most 256. Codes and the rows of queries, keys and values start on
  * 16 bytes. Block ids outside [0, NB) are read as blocks that hold nothing and
  * are never written. All calls only queue kernels and can be captured.
+ * Scales are positive normal numbers. Sums of values are held in fp32 relative
+ * to a maximum that may lag by 2^8: cached values beyond 2^96 may overflow them.
  */
 #define KVX_DTYPE_BF16 0
 #define KVX_DTYPE_FP16 1
@@ -214,9 +216,10 @@ typedef struct kvx_paged_batch {
   const int32_t* context_lens;
   const int32_t* cu_seqlens; /* NULL: one row a sequence, or none in the call (num_tokens 0) */
   int64_t table_stride;      /* elements */
-  int32_t table_width;       /* blocks of a table */
+  int32_t table_width;       /* blocks of a table; attention's launch is sized by it */
   int32_t num_seqs;
-  int32_t max_seqlen; /* the most rows of a sequence; a launch is sized by it, and longer ones are computed too */
+  int32_t max_seqlen; /* the most rows of a sequence; a launch is sized by it and its kernel chosen by it, and longer
+                         ones are computed too, as exactly, in more time */
   int32_t num_tokens; /* rows of the call; those of no sequence are not written */
 } kvx_paged_batch;
 

@@ -491,8 +491,9 @@ __global__ __launch_bounds__(kThreads, kHd * kTiles <= 128 ? 2 : 1) void few_row
 // The maximum that exponents are taken from moves only when a score exceeds it
 // by 2^8: P <= 2^8 costs bf16 and fp32 no precision, and most steps need neither
 // a reduction over lanes nor a pass over the outputs.
-// Two chunks (3,549 rows of 32 heads of 128) behind 6-8 K tokens take 476 us, 780
-// TFLOP/s; 30% of the issue slots are matrix instructions', 50% other arithmetic's.
+// Two chunks (3,549 rows of 32 heads of 128) behind 6-8 K tokens take 592 us, 627
+// TFLOP/s; the matrix cores are busy for 52% of the time, with three products for
+// each two that count, and arithmetic takes 60% of the issue cycles.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(kWaves* kWave) void chunk_kernel(AttentionArgs a) {
       }
       u32x4 p[2][2];  // P to bf16, and what the rounding left
       // The wave that has scores and exponentials to issue goes first, so that the SIMD's two waves fall out of step and
-      // one's outputs run under the other's exponentials: 477 us in place of 511 for two chunks behind 6-8 K tokens.
+      // one's outputs run under the other's exponentials: 551 us in place of 599 for two chunks behind 6-8 K tokens.
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < kTurns; ++t) {
@@ -1282,7 +1283,7 @@ __global__ __launch_bounds__(kThreads, kHd < 256 ? 3 : 2) void weights_many_kern
 int padded_head(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 // Query rows of one (sequence, KV head) up to which the few-rows kernel runs (16 contexts of 4 K tokens on 8 heads, 32
-// rows: 64 us, the chunk kernel 75; 48 rows: 148 and 79).
+// rows: 65 us, the chunk kernel 83; 48 rows: 150 and 87).
 constexpr int kFewRows = 32;
 int few_tiles(int64_t rows, int padded) { return rows <= 16 || padded == 256 ? 1 : 2; }
 constexpr int kChunkWaves = 8;
@@ -1375,12 +1376,14 @@ AttentionPlan attention_plan(const Fp8Cache& c, const PagedBatch& b, int32_t q_h
   const int64_t groups = (int64_t)b.num_seqs * c.heads * plan.row_tiles;
   const int64_t steps = ((int64_t)b.table_width * c.block_size + kStep - 1) / kStep;
   // Split the keys while there are too few workgroups to fill the chip, each keeping 256 keys or more (1,024: 16 chunks of
-  // 6 tokens and 8 query heads over 4 K 34.6 us, now 19.2). Chunks: up to one workgroup a CU, which is what one has LDS
-  // for (up to two, 256 of a chunk of 2,048 tokens over 8 K took 393 us, now 278; 160 of shorter ones 152 and 78).
+  // 6 tokens and 8 query heads over 4 K 40 us, now 20). Chunks: up to one workgroup a CU, which is what one has LDS
+  // for (up to two, 256 of a chunk of 2,048 tokens over 8 K took 472 us, now 360; 160 of 1,280 over 4 K 204 and 162).
   // Few rows: with few (sequence, KV head) pairs, one workgroup a CU, as the join takes its time for each split (8 pairs of
-  // 32 K tokens in 128 / 64 / 32 / 16 splits 23.7 / 21.6 / 19.8 / 25.7 us); with more, some for each CU (64 pairs of 8 K in
-  // 32 / 16 33.5 / 30.4); with many, so many that contexts of unlike lengths even out (61 of 300 to 8,192 tokens on 8 heads
-  // in 4 / 8 splits 114 / 105; 2,048 pairs of 2 K in 2 / 1 219 / 203).
+  // 32 K tokens in 128 / 64 / 32 / 16 splits 23.7 / 21.6 / 19.8 / 25.7 us); with many, so many that contexts of unlike
+  // lengths even out (61 of 300 to 8,192 tokens on 8 heads in 4 / 8 splits 114 / 105; 2,048 pairs of 2 K in 2 / 1 219 /
+  // 193). About the borders, with contexts all of one length and 256 / 1,024 / 4,096 workgroups: 15 pairs of 8 K 13.3 / 14.5
+  // / 14.5 us, 16 13.4 / 14.6 / 14.6, 32 18.6 / 23.7 / 23.6, 192 94 / 79 / 85, 240 97 / 100 / 103, 320 131 / 129 / 130;
+  // 1,920 pairs of 2 K 185 / 186 / 206, 2,560 240 in each. Where all are as long, fewer splits would mostly do.
   const int64_t want = !few || groups < 16 ? 256 : groups < 256 ? 1024 : groups < 2048 ? 4096 : groups;
   const int64_t unit = few ? 8 : chunk_keys(padded_head(c.head_dim)) / kStep, least = 8;
   int64_t splits = want / groups;

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void store_fp8_kernel(Fp8Cache c, const T
 // weights a lane stay in registers throughout, so that two bits cost three
 // comparisons and scalar bit counts for each 64 weights and one barrier (bit by
 // bit, the barriers made it 18.6 and 33.1 us for rows of 8,192 and 32,767); rows
-// of more than 32,768 are read again for each two. The search ends early where exactly as
+// of more than 32,768 are read again for each two (32,768: 33 us, 32,769: 91, 102,400: 308). The search ends early where exactly as
 // many are reached as wanted, and leaves out bits that all patterns share. (A
 // radix select by histograms in LDS took 21 and 46 us for rows of 8,192 and
 // 32,767: weights crowd in few bins, and additions to one address take turns.)
@@ -629,8 +629,9 @@ hipError_t rotary_of(const RotaryArgs& a, hipStream_t stream) {
 // of 16 take 27 us by one wave and 52 by four, in groups of 32 28.5 by two and 34.5 by four.
 // Each looks at as many tokens as leave so many workgroups, and at most at a group's, so that most of a prompt's find one
 // group that begins. A decode step's tokens begin a group each, which then wait for one another: with 2,048 / 4,096 / 8,192
-// workgroups of one wave 1,024 appended tokens of 8 heads take 20.7 / 13.9 / 14.4 us, as many of a prompt 6.6 / 8.6 / 14.3;
-// with 2,048 / 4,096 of more waves, in groups of 64, 41 / 41 and (4,096 tokens of a prompt) 15 / 26.
+// workgroups of one wave 1,024 appended tokens of 8 heads take 21.1 / 14.3 / 14.7 us, as many of a prompt 6.7 / 8.6 / 13.1
+// (512: 12.3 / 9.1 / 10.0 and 6.6 / 8.3 / 9.8; 2,048: 38.9 / 24.3 / 24.4 and 6.9 / 8.7 / 13.6); with 1,024 / 2,048 / 4,096
+// of four, in groups of 64, 43 / 42 / 42 and 8.3 / 13.2 / 15.1 (4,096 tokens: 162 / 156 / 148 and 8.9 / 15.0 / 25.2).
 constexpr int kStoreFull = 4096, kStoreFullWide = 2048;
 
 template <typename T, int kThreads>

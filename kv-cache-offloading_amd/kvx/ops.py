@@ -528,8 +528,11 @@ def attention_fp8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     a sequence's blocks are not read, ids outside the pool count as blocks without tokens.
 
     Decode: N == B, row b is sequence b's newest token. Chunks: cu_seqlens, int32 [B + 1], row range of each sequence
-    (row i of n sees the tokens up to context - n + i) and max_seqlen, the most rows of one (a hint that sizes the
-    launch; default N). Rows of no sequence are left as they are; rows that see no token become 0. out: contiguous
+    (row i of n sees the tokens up to context - n + i) and max_seqlen, the most rows of one: a hint that sizes the
+    launch and changes no result by more than its rounding. It defaults to N, which costs time where many sequences
+    have few rows each (64 of 3 rows over 4,096 tokens of 8 heads: 310 us, with the hint 130); the width of
+    block_tables sizes the launch likewise (one row over 2,048 tokens of 8 heads: 10 us, in tables of 131,072 tokens
+    24). Rows of no sequence are left as they are; rows that see no token become 0. out: contiguous
     [N, q_heads, head_dim] of the query's type; lse: float32 [N, q_heads], log of the sum of exp(scores), -inf for
     rows that see no token. softmax_scale, positive, defaults to head_dim ** -0.5. Capturable in a HIP graph.
     """
